@@ -275,6 +275,85 @@ int mes_awq_gemm_on_panel(int epilogue, const void* X, int64_t ldx, const void* 
                           const void* bias, void* Y, int64_t ldy, int64_t M, int64_t N,
                           int64_t K, void* stream);
 
+/* ---------------------------------------------------------------------------------
+ * Token steps: extending sequences that have been seen before.  No counterparts in the
+ * reference, which runs every sequence from its first token.
+ * ------------------------------------------------------------------------------- */
+
+/* Y = X * W for 1 to 16 rows: the projections of a token step.  `epilogue` as for
+ * mes_awq_gemm_ws: 0 Y bf16 [M, N] = X W (+ bias), 1 Y f32 [M, N] += X W (+ bias), 2 Y bf16
+ * [M, N/2] = silu(gate) * up with gate and up columns interleaved in blocks of 16 (bias NULL).
+ * W = (q - z) * s is used exactly (mes_awq_gemm rounds it to bf16 first); fp32 accumulation in
+ * a fixed order.  X: bf16 [M, K], pitch ldx elements; qweight_mes, qzeros, scales, bias as for
+ * mes_awq_gemm.  group_size 32, 64 or 128; K % 128 == 0; N % 8 == 0 (N % 32 == 0 for
+ * epilogue 2); ldx % 8 == 0.  X and qweight_mes 16-byte aligned, scales 8, qzeros 4, Y to its
+ * elements.  M = 0 does nothing; M > 16 is MES_ERR_INVALID. */
+int mes_awq_gemv(int epilogue, const void* X, int64_t ldx, const int32_t* qweight_mes,
+                 const int32_t* qzeros, const void* scales, const void* bias, void* Y,
+                 int64_t ldy, int64_t M, int64_t N, int64_t K, int group_size, void* stream);
+
+/* Paged KV cache held in 8 bits.
+ *   codes   [num_pages][2][Hkv][P][D] bytes (K, then V): int8 (dtype 0) or e4m3 (dtype 1)
+ *   scales  f32 [num_pages][2][Hkv]: value = code * scale, one scale for a page, side and head
+ *   sums    f32 [num_pages][Hkv][P]: accumulated attention weights, optional (NULL)
+ *   block_table i32 [B][table_width]: page of token t of sequence b = block_table[b][t / P],
+ *           slot t % P.  Entries past a sequence's last page are not read.
+ *   cu_new  i32 [B + 1]: offsets of each sequence's new tokens in the packed rows [T]
+ *   context_lens i32 [B]: cached tokens of each sequence, the new ones among them, so new token
+ *           i of sequence b is token context_lens[b] - (cu_new[b+1] - cu_new[b]) + i
+ * D == 128; P = page_size is 16, 32, 64 or 128; num_pages * 2 * Hkv * P < 2^31 rows.
+ * max_new: an upper bound on the new tokens of one sequence, known to the host.  Lengths and
+ * pages are read on the device; ones that lie outside T, the table or the cache are skipped and
+ * record MES_ERR_INVALID as device error.  Sequences must not share pages that are written. */
+
+/* Quantises new keys and values into the cache.  K, V: bf16 rows of pitch ldk / ldv elements,
+ * Hkv heads of D.  The scale of a (page, side, head) becomes max(old, amax|new| / Q), Q = 127
+ * (int8) or 448 (e4m3), where old counts only if the page held tokens before; when it grows,
+ * the older tokens' codes become rne(code * old / scale).  New codes are rne(x / scale).
+ * Infinities saturate and do not set the scale; NaN is stored as 0.  With sums, the new tokens'
+ * sums are set to 0.  codes 16-byte aligned, K and V too. */
+int mes_kv8_append(int dtype, const void* K, int64_t ldk, const void* V, int64_t ldv,
+                   void* codes, float* scales, float* sums, const int32_t* block_table,
+                   int64_t table_width, const int32_t* cu_new, const int32_t* context_lens,
+                   int64_t B, int64_t T, int64_t max_new, int Hkv, int D, int page_size,
+                   int64_t num_pages, void* stream);
+
+/* out[i] = the values of pages[i], bf16 [n][2][Hkv][P][D].  A page outside the cache gives zeros
+ * and records MES_ERR_INVALID. */
+int mes_kv8_read(int dtype, const void* codes, const float* scales, const int32_t* pages,
+                 int64_t n, int Hkv, int D, int page_size, int64_t num_pages, void* out,
+                 void* stream);
+
+/* Causal grouped-query attention of the new tokens over the cache (their own keys and values
+ * included, so append first).  q: bf16 rows of pitch ldq elements, Hq heads of D, Hq % Hkv == 0;
+ * out: bf16 [T][Hq * D].  A token that sees nothing gives zeros.  With sums, every cached
+ * token's weight, summed over the new tokens and the query heads of its kv head, is added to its
+ * sum.  At most 1024 sequences.  workspace: 256-byte aligned, of
+ * mes_kv8_attention_workspace_size(T, B, Hq, Hkv, max_new, max_context) bytes, max_context =
+ * table_width * P with sums and 0 without; its contents are undefined after the call. */
+int64_t mes_kv8_attention_workspace_size(int64_t T, int64_t B, int Hq, int Hkv, int64_t max_new,
+                                         int64_t max_context);
+int mes_kv8_attention(int dtype, const void* q, int64_t ldq, const void* codes,
+                      const float* scales, float* sums, const int32_t* block_table,
+                      int64_t table_width, const int32_t* cu_new, const int32_t* context_lens,
+                      int64_t B, int64_t T, int64_t max_new, int Hq, int Hkv, int D,
+                      int page_size, int64_t num_pages, float scale, void* out, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
+/* Cuts every sequence down to `keep` tokens: its last `recent` ones (recent <= keep) and, for
+ * each kv head by itself, those of the others whose sums are largest (a tie goes to the earlier
+ * token, NaN ranks lowest), in their order.  The kept tokens are copied, codes and sums, to the
+ * pages of new_table i32 [B][new_width], new_width = ceil(keep / P), which must not be among the
+ * sequences' present pages.  A new page's scale is the largest of its tokens' scales; a token
+ * whose own scale is smaller becomes rne(code * own / scale).  Slots past the last token hold
+ * code 0.  kept: i32 [B][Hkv][keep], the tokens kept (-1 past the end); new_lens: i32 [B],
+ * min(context_lens, keep).  A sequence of at most `keep` tokens is copied whole. */
+int mes_kv8_evict(int dtype, void* codes, float* scales, float* sums,
+                  const int32_t* block_table, int64_t table_width, const int32_t* context_lens,
+                  int64_t B, const int32_t* new_table, int64_t new_width, int64_t keep,
+                  int64_t recent, int Hkv, int D, int page_size, int64_t num_pages,
+                  int32_t* kept, int32_t* new_lens, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

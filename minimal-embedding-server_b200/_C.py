@@ -55,6 +55,16 @@ SIGNATURES = {
     "mes_awq_gemm_on_panel": (_i32, [_i32, _vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp]),
     "mes_awq_gemm_ws": (_i32, [_i32, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64,
                                _i32, _vp, _i64, _vp]),
+    "mes_awq_gemv": (_i32, [_i32, _vp, _i64, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _i32,
+                            _vp]),
+    "mes_kv8_append": (_i32, [_i32, _vp, _i64, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64,
+                              _i64, _i64, _i32, _i32, _i32, _i64, _vp]),
+    "mes_kv8_read": (_i32, [_i32, _vp, _vp, _vp, _i64, _i32, _i32, _i32, _i64, _vp, _vp]),
+    "mes_kv8_attention_workspace_size": (_i64, [_i64, _i64, _i32, _i32, _i64, _i64]),
+    "mes_kv8_attention": (_i32, [_i32, _vp, _i64, _vp, _vp, _vp, _vp, _i64, _vp, _vp, _i64, _i64,
+                                 _i64, _i32, _i32, _i32, _i32, _i64, _f32, _vp, _vp, _i64, _vp]),
+    "mes_kv8_evict": (_i32, [_i32, _vp, _vp, _vp, _vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64,
+                             _i32, _i32, _i32, _i64, _vp, _vp, _vp]),
 }
 
 _lib = None
@@ -499,3 +509,174 @@ def awq_gemm(x: torch.Tensor, qweight_mes: torch.Tensor, qzeros: torch.Tensor,
         out = torch.empty(M, N, dtype=torch.bfloat16, device=x.device)
     _awq_gemm_call(EPI_BF16, x, qweight_mes, qzeros, scales, bias, out, group_size, panel)
     return out
+
+
+# --------------------------------------------------------------------------------------
+# Token steps: matrix-vector products and the 8-bit paged KV cache
+# --------------------------------------------------------------------------------------
+GEMV_MAX_ROWS = 16
+
+
+def _awq_gemv_call(epi: int, x: torch.Tensor, qweight_mes: torch.Tensor, qzeros: torch.Tensor,
+                   scales: torch.Tensor, bias, y: torch.Tensor, group_size: int) -> None:
+    _awq_args(qweight_mes, qzeros, scales, x, group_size)
+    K, N = qweight_mes.shape[0] * 8, qweight_mes.shape[1]
+    _arg(bias, "bias", x, torch.bfloat16, (N,), contiguous=True)
+    _check(lib().mes_awq_gemv(epi, _p(x), x.stride(0), _p(qweight_mes), _p(qzeros), _p(scales),
+                              _p(bias), _p(y), y.stride(0), x.shape[0], N, K, group_size,
+                              _stream(x)), f"mes_awq_gemv ({_EPI_NAME[epi]} epilogue)")
+
+
+def _gemv_x(x: torch.Tensor, qweight_mes: torch.Tensor) -> None:
+    _need(x.dtype == torch.bfloat16 and x.dim() == 2 and x.stride(-1) == 1,
+          "x must be bf16 [M, K] with unit inner stride")
+    _need(x.shape[0] <= GEMV_MAX_ROWS, f"x has {x.shape[0]} rows, at most {GEMV_MAX_ROWS} are taken")
+    _need(qweight_mes.dim() == 2 and x.shape[1] == qweight_mes.shape[0] * 8,
+          f"x has K={x.shape[1]}, weight has K={qweight_mes.shape[0] * 8}")
+
+
+def awq_gemv(x: torch.Tensor, qweight_mes: torch.Tensor, qzeros: torch.Tensor,
+             scales: torch.Tensor, bias: torch.Tensor | None = None,
+             out: torch.Tensor | None = None, group_size: int = 128) -> torch.Tensor:
+    """``x[M, K] @ W[K, N] (+ bias)`` for at most 16 rows: the projections of a token step
+    (``mes_awq_gemv``).  The weights are not rounded to bf16 first, as ``awq_gemm`` does."""
+    _gemv_x(x, qweight_mes)
+    M, N = x.shape[0], qweight_mes.shape[1]
+    _arg(out, "out", x, torch.bfloat16, (M, N), unit_stride=True)
+    if out is None:
+        out = torch.empty(M, N, dtype=torch.bfloat16, device=x.device)
+    _awq_gemv_call(EPI_BF16, x, qweight_mes, qzeros, scales, bias, out, group_size)
+    return out
+
+
+def awq_gemv_residual(x: torch.Tensor, qweight_mes: torch.Tensor, qzeros: torch.Tensor,
+                      scales: torch.Tensor, residual: torch.Tensor,
+                      bias: torch.Tensor | None = None, group_size: int = 128) -> torch.Tensor:
+    """``residual[M, N] (fp32) += x @ W (+ bias)`` for at most 16 rows."""
+    _gemv_x(x, qweight_mes)
+    _arg(residual, "residual", x, torch.float32, (x.shape[0], qweight_mes.shape[1]), unit_stride=True)
+    _awq_gemv_call(EPI_RESIDUAL, x, qweight_mes, qzeros, scales, bias, residual, group_size)
+    return residual
+
+
+def awq_gemv_silu(x: torch.Tensor, qweight_mes: torch.Tensor, qzeros: torch.Tensor,
+                  scales: torch.Tensor, out: torch.Tensor | None = None,
+                  group_size: int = 128) -> torch.Tensor:
+    """``silu(x @ Wg) * (x @ Wu)`` for at most 16 rows, gate/up columns interleaved in blocks of
+    16 (see ``interleave_gate_up``); output ``[M, N/2]`` bf16."""
+    _gemv_x(x, qweight_mes)
+    M, N = x.shape[0], qweight_mes.shape[1]
+    _arg(out, "out", x, torch.bfloat16, (M, N // 2), unit_stride=True)
+    if out is None:
+        out = torch.empty(M, N // 2, dtype=torch.bfloat16, device=x.device)
+    _awq_gemv_call(EPI_SILU, x, qweight_mes, qzeros, scales, None, out, group_size)
+    return out
+
+
+KV8_DTYPES = {torch.int8: 0, torch.float8_e4m3fn: 1}
+KV8_PAGE_SIZES = (16, 32, 64, 128)
+
+
+def _kv8_cache(codes: torch.Tensor, scales: torch.Tensor, sums: torch.Tensor | None = None):
+    """``(dtype code, num_pages, Hkv, P, D)`` of a cache ``codes [pages, 2, Hkv, P, 128]``,
+    ``scales [pages, 2, Hkv]``, ``sums [pages, Hkv, P]``."""
+    kind = KV8_DTYPES.get(codes.dtype)
+    _need(kind is not None and codes.dim() == 5, "codes must be int8 or float8_e4m3fn [pages, 2, Hkv, P, 128]")
+    pages, two, Hkv, P, D = codes.shape
+    _need(two == 2 and P in KV8_PAGE_SIZES and D == 128 and codes.is_contiguous(),
+          "codes must be contiguous [pages, 2, Hkv, P, 128] with P one of 16, 32, 64, 128")
+    _arg(scales, "scales", codes, torch.float32, (pages, 2, Hkv), contiguous=True)
+    _arg(sums, "sums", codes, torch.float32, (pages, Hkv, P), contiguous=True)
+    return kind, pages, Hkv, P, D
+
+
+def _kv8_batch(block_table: torch.Tensor, context_lens: torch.Tensor, like: torch.Tensor) -> int:
+    """Checks ``block_table [B, width]`` and ``context_lens [B]`` (int32); returns B."""
+    _need(block_table.dim() == 2, "block_table must be int32 [B, width]")
+    B = block_table.shape[0]
+    _arg(block_table, "block_table", like, torch.int32, contiguous=True)
+    _arg(context_lens, "context_lens", like, torch.int32, (B,), contiguous=True)
+    return B
+
+
+def kv8_append(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
+               block_table: torch.Tensor, cu_new: torch.Tensor, context_lens: torch.Tensor,
+               max_new: int, sums: torch.Tensor | None = None) -> None:
+    """Quantise the new tokens' ``k`` / ``v`` (bf16 rows ``[T, Hkv * 128]``, e.g. columns of the
+    packed QKV buffer) into the cache (``mes_kv8_append``).  ``cu_new`` int32 ``[B + 1]``:
+    offsets of each sequence's rows; ``context_lens`` counts the cached tokens with the new
+    ones; ``max_new``: no sequence has more new tokens."""
+    kind, pages, Hkv, P, D = _kv8_cache(codes, scales, sums)
+    B = _kv8_batch(block_table, context_lens, codes)
+    _need(k.dim() == 2, "k must be bf16 [T, Hkv * 128]")
+    T = k.shape[0]
+    _arg(k, "k", codes, torch.bfloat16, (T, Hkv * D), unit_stride=True)
+    _arg(v, "v", codes, torch.bfloat16, (T, Hkv * D), unit_stride=True)
+    _arg(cu_new, "cu_new", codes, torch.int32, (B + 1,), contiguous=True)
+    _check(lib().mes_kv8_append(kind, _p(k), k.stride(0), _p(v), v.stride(0), _p(codes), _p(scales),
+                                _p(sums), _p(block_table), block_table.shape[1], _p(cu_new),
+                                _p(context_lens), B, T, max_new, Hkv, D, P, pages, _stream(codes)),
+           "mes_kv8_append")
+
+
+def kv8_read(codes: torch.Tensor, scales: torch.Tensor, pages: torch.Tensor,
+             out: torch.Tensor | None = None) -> torch.Tensor:
+    """The values of ``pages`` (int32 ``[n]``), bf16 ``[n, 2, Hkv, P, 128]``."""
+    kind, num_pages, Hkv, P, D = _kv8_cache(codes, scales)
+    _need(pages.dim() == 1, "pages must be int32 [n]")
+    _arg(pages, "pages", codes, torch.int32, contiguous=True)
+    n = pages.shape[0]
+    _arg(out, "out", codes, torch.bfloat16, (n, 2, Hkv, P, D), contiguous=True)
+    if out is None:
+        out = torch.empty(n, 2, Hkv, P, D, dtype=torch.bfloat16, device=codes.device)
+    _check(lib().mes_kv8_read(kind, _p(codes), _p(scales), _p(pages), n, Hkv, D, P, num_pages, _p(out),
+                              _stream(codes)), "mes_kv8_read")
+    return out
+
+
+def kv8_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
+                  block_table: torch.Tensor, cu_new: torch.Tensor, context_lens: torch.Tensor,
+                  num_heads: int, scale: float, max_new: int, out: torch.Tensor | None = None,
+                  sums: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of the new tokens' ``q`` (bf16 rows ``[T, num_heads * 128]``) over the
+    cache, their own entries included (``mes_kv8_attention``); bf16 ``[T, num_heads * 128]``.
+    With ``sums``, the cached tokens' attention weights are added to it."""
+    kind, pages, Hkv, P, D = _kv8_cache(codes, scales, sums)
+    B = _kv8_batch(block_table, context_lens, codes)
+    _need(q.dim() == 2, "q must be bf16 [T, num_heads * 128]")
+    T, width = q.shape[0], block_table.shape[1]
+    _arg(q, "q", codes, torch.bfloat16, (T, num_heads * D), unit_stride=True)
+    _arg(cu_new, "cu_new", codes, torch.int32, (B + 1,), contiguous=True)
+    _arg(out, "out", codes, torch.bfloat16, (T, num_heads * D), contiguous=True)
+    if out is None:
+        out = torch.empty(T, num_heads * D, dtype=torch.bfloat16, device=codes.device)
+    size = int(lib().mes_kv8_attention_workspace_size(T, B, num_heads, Hkv, max_new,
+                                                      0 if sums is None else width * P))
+    _need(size >= 0, f"unsupported sizes: {T} tokens of {B} sequences (at most {max_new} of one), "
+                     f"{num_heads} heads over {Hkv}")
+    ws = torch.empty(size, dtype=torch.uint8, device=codes.device)
+    _check(lib().mes_kv8_attention(kind, _p(q), q.stride(0), _p(codes), _p(scales), _p(sums),
+                                   _p(block_table), width, _p(cu_new), _p(context_lens), B, T,
+                                   max_new, num_heads, Hkv, D, P, pages, scale, _p(out), _p(ws), size,
+                                   _stream(codes)), "mes_kv8_attention", 2 if sums is None else 3)
+    return out
+
+
+def kv8_evict(codes: torch.Tensor, scales: torch.Tensor, sums: torch.Tensor,
+              block_table: torch.Tensor, context_lens: torch.Tensor, new_table: torch.Tensor,
+              keep: int, recent: int):
+    """Copy each sequence's ``recent`` last tokens and its tokens of largest ``sums`` (per kv
+    head), ``keep`` in all, to the pages of ``new_table`` int32 ``[B, ceil(keep / P)]``
+    (``mes_kv8_evict``).  Returns ``(kept int32 [B, Hkv, keep], new_lens int32 [B])``."""
+    kind, pages, Hkv, P, D = _kv8_cache(codes, scales, sums)
+    _need(sums is not None, "sums must be float32 [pages, Hkv, P]")
+    B = _kv8_batch(block_table, context_lens, codes)
+    _need(0 <= recent <= keep and keep > 0, "0 <= recent <= keep, keep > 0")
+    _arg(new_table, "new_table", codes, torch.int32, (B, -(-keep // P)), contiguous=True)
+    kept = torch.empty(B, Hkv, keep, dtype=torch.int32, device=codes.device)
+    new_lens = torch.empty(B, dtype=torch.int32, device=codes.device)
+    _check(lib().mes_kv8_evict(kind, _p(codes), _p(scales), _p(sums), _p(block_table),
+                               block_table.shape[1], _p(context_lens), B, _p(new_table),
+                               new_table.shape[1], keep, recent, Hkv, D, P, pages, _p(kept), _p(new_lens),
+                               _stream(codes)), "mes_kv8_evict", 2)
+    return kept, new_lens

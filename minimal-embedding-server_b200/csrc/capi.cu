@@ -10,6 +10,8 @@
 extern "C" int mes_elementwise_take_error(int* code);
 extern "C" int mes_gemm_take_error(int* code);
 extern "C" int mes_attention_take_error(int* code);
+extern "C" int mes_kv8_cache_take_error(int* code);
+extern "C" int mes_kv8_attention_take_error(int* code);
 
 namespace mes_host {
 
@@ -132,7 +134,8 @@ extern "C" int mes_take_device_error(int* code) {
   if (!code) return MES_ERR_INVALID;
   *code = 0;
   if (cudaDeviceSynchronize() != cudaSuccess) return MES_ERR_CUDA;
-  int (*fns[3])(int*) = {mes_elementwise_take_error, mes_gemm_take_error, mes_attention_take_error};
+  int (*fns[])(int*) = {mes_elementwise_take_error, mes_gemm_take_error, mes_attention_take_error,
+                        mes_kv8_cache_take_error, mes_kv8_attention_take_error};
   for (auto f : fns) {
     int c = 0;
     int st = f(&c);

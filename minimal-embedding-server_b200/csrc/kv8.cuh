@@ -1,0 +1,46 @@
+// The 8-bit paged KV cache: layout, element types and what its kernels share.
+//
+// codes [pages][2][Hkv][P][128] (K, then V) one byte each, scales f32 [pages][2][Hkv], optional
+// sums f32 [pages][Hkv][P]; value = code * scale.  P tokens of one head and side are one run of
+// P * 128 bytes with one scale, so a run is the unit of quantisation and of the copies.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+
+namespace kv8 {
+
+constexpr int kD = 128;
+
+enum Kind { kInt8 = 0, kE4m3 = 1 };
+
+template <int kKind>
+__host__ __device__ constexpr float code_max() {
+  return kKind == kInt8 ? 127.0f : 448.0f;
+}
+
+// Value over its scale -> code, to nearest even within the finite range; NaN -> 0.
+template <int kKind>
+__device__ __forceinline__ uint32_t encode(float x) {
+  x = x == x ? x : 0.f;
+  x = fminf(fmaxf(x, -code_max<kKind>()), code_max<kKind>());
+  if (kKind == kInt8) return static_cast<uint32_t>(__float2int_rn(x)) & 0xffu;
+  return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+}
+template <int kKind>
+__device__ __forceinline__ float decode(uint32_t code) {
+  if (kKind == kInt8) return static_cast<float>(static_cast<int8_t>(code & 0xffu));
+  return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(code & 0xffu), __NV_E4M3)));
+}
+
+// Host checks shared by the entry points.
+inline bool aligned(const void* p, uintptr_t a) { return (reinterpret_cast<uintptr_t>(p) & (a - 1)) == 0; }
+inline bool valid_cache(int dtype, int64_t num_pages, int Hkv, int D, int page) {
+  return (dtype == kInt8 || dtype == kE4m3) && D == kD && Hkv > 0 && Hkv <= 1024 && num_pages > 0 &&
+         (page == 16 || page == 32 || page == 64 || page == 128) &&
+         // rows of 128 bytes are counted in 32 bits (256 GB of codes)
+         num_pages <= 0x7fffffffll / (2ll * Hkv * page);
+}
+
+}  // namespace kv8

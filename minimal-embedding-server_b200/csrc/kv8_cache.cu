@@ -1,0 +1,525 @@
+// Writing, reading back and compacting the 8-bit paged KV cache (layout: kv8.cuh).  All three
+// move bytes: their bound is what they read and write.
+#include "kv8.cuh"
+
+namespace {
+
+__device__ int g_err_kv8_cache = 0;
+
+__device__ __forceinline__ void record(int code) { atomicCAS(&g_err_kv8_cache, 0, code); }
+
+__device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
+  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&v);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 t = __bfloat1622float2(h[i]);
+    f[2 * i] = t.x;
+    f[2 * i + 1] = t.y;
+  }
+}
+
+// Rows of one run handled by a warp, and the block shape that follows: a run of P tokens takes
+// P / 16 warps, and a block holds at least four warps, so small pages share a block.
+constexpr int kWarpRows = 16;
+template <int P>
+struct Shape {
+  static constexpr int kRunWarps = P / kWarpRows;
+  static constexpr int kRuns = kRunWarps < 4 ? 4 / kRunWarps : 1;   // runs of a block
+  static constexpr int kThreads = 32 * kRunWarps * kRuns;
+};
+
+// Largest value over the warps of a run; every thread of the block calls it.
+template <int P>
+__device__ __forceinline__ float run_max(float v, float* red) {
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+  if (Shape<P>::kRunWarps == 1) return v;
+  const int warp = threadIdx.x >> 5, first = warp / Shape<P>::kRunWarps * Shape<P>::kRunWarps;
+  if ((threadIdx.x & 31) == 0) red[warp] = v;
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < Shape<P>::kRunWarps; ++i) v = fmaxf(v, red[first + i]);
+  return v;
+}
+
+// ----------------------------------------- append --------------------------------------
+// Run (sequence b, touched page j, side, head): s = max(s_old, amax|new| / Q), old tokens of the
+// run re-rounded when s grew, new tokens rounded once.  s_old counts only where the run already
+// held tokens.  Non-finite inputs do not set the scale: an infinity saturates, NaN becomes 0.
+// Each new value is read once and kept in registers between the maximum and the rounding.
+template <int kKind, int P>
+__global__ void __launch_bounds__(Shape<P>::kThreads)
+kv8_append_kernel(const __nv_bfloat16* __restrict__ Kn, int64_t ldk, const __nv_bfloat16* __restrict__ Vn,
+                  int64_t ldv, uint8_t* codes, float* scales, float* sums,
+                  const int32_t* __restrict__ table, int64_t width, const int32_t* __restrict__ cu,
+                  const int32_t* __restrict__ ctx, int64_t T, int max_pages, int Hkv,
+                  int64_t num_pages) {
+  __shared__ float red[8];
+  constexpr float kQ = kv8::code_max<kKind>();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t b = blockIdx.x / max_pages;
+  const int j = blockIdx.x - static_cast<int>(b * max_pages);
+  const int run = blockIdx.y * Shape<P>::kRuns + warp / Shape<P>::kRunWarps;
+  const int side = run >= Hkv, h = run - side * Hkv;
+  const int r0 = cu[b], n = cu[b + 1] - r0, len = ctx[b], start = len - n;
+  bool ok = run < 2 * Hkv && n > 0;
+  const bool sane = r0 >= 0 && n >= 0 && start >= 0 && r0 + (int64_t)n <= T && (int64_t)len <= width * P;
+  const int p = sane ? start / P + j : 0;
+  ok = ok && sane && (int64_t)p * P < len;
+  int64_t page = 0;
+  if (ok) {
+    page = table[b * width + p];
+    if (page < 0 || page >= num_pages) {
+      ok = false;
+      if (threadIdx.x == 0) record(MES_ERR_INVALID);
+    }
+  }
+  if (threadIdx.x == 0 && blockIdx.y == 0) {
+    // A sequence with more new tokens than the grid has pages for is an error of the caller.
+    if (!sane || (j == 0 && n > 0 && (len - 1) / P - start / P >= max_pages)) record(MES_ERR_INVALID);
+  }
+  const __nv_bfloat16* src = side ? Vn : Kn;
+  const int64_t ld = side ? ldv : ldk;
+  const int slot0 = warp % Shape<P>::kRunWarps * kWarpRows + (lane >> 4), col = (lane & 15) * 8;
+  uint4 x[8];
+  float amax = 0.f;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int t = p * P + slot0 + 2 * i;
+    x[i] = make_uint4(0, 0, 0, 0);
+    if (ok && t >= start && t < len)
+      x[i] = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)(r0 + t - start) * ld + h * kv8::kD + col));
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    float f[8];
+    unpack8(x[i], f);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float a = fabsf(f[e]);
+      amax = a <= 3.4028235e38f ? fmaxf(amax, a) : amax;
+    }
+  }
+  const int64_t si = (page * 2 + side) * Hkv + h;
+  const float was = ok && p * P < start ? scales[si] : 0.f;
+  amax = run_max<P>(amax, red);
+  __syncthreads();                      // every warp of the run has read the old scale
+  if (!ok) return;
+  const float now = fmaxf(was, amax / kQ), safe = now > 0.f ? now : 1.f;
+  uint8_t* dst = codes + si * P * kv8::kD;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const int slot = slot0 + 2 * i, t = p * P + slot;
+    if (t >= len || (t < start && !(now > was))) continue;
+    uint2* at = reinterpret_cast<uint2*>(dst + slot * kv8::kD + col);
+    float f[8];
+    if (t >= start) {
+      unpack8(x[i], f);
+    } else {
+      const uint2 old = *at;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        f[e] = kv8::decode<kKind>((e < 4 ? old.x : old.y) >> (8 * (e & 3))) * was;
+    }
+    uint32_t o[2] = {0, 0};
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e >> 2] |= kv8::encode<kKind>(f[e] / safe) << (8 * (e & 3));
+    *at = make_uint2(o[0], o[1]);
+    if (sums && side == 0 && t >= start && col == 0) sums[(page * Hkv + h) * P + slot] = 0.f;
+  }
+  if (lane == 0 && warp % Shape<P>::kRunWarps == 0) scales[si] = now;
+}
+
+// ------------------------------------------ read ---------------------------------------
+// out[i] = code * scale of pages[i], rounded to bf16: one 16-byte load and two 16-byte stores a
+// thread.
+template <int kKind>
+__global__ void kv8_read_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ scales,
+                                const int32_t* __restrict__ pages, int64_t chunks, int64_t page_chunks,
+                                int64_t run_chunks, int64_t num_pages, uint4* __restrict__ out) {
+  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < chunks;
+       i += (int64_t)gridDim.x * blockDim.x) {
+    const int64_t n = i / page_chunks, r = i - n * page_chunks;
+    const int64_t page = __ldg(pages + n);
+    uint4 o[2] = {};
+    if (page < 0 || page >= num_pages) {
+      if (r == 0) record(MES_ERR_INVALID);
+    } else {
+      const uint4 v = __ldg(reinterpret_cast<const uint4*>(codes) + page * page_chunks + r);
+      const float s = __ldg(scales + page * (page_chunks / run_chunks) + r / run_chunks);
+      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+      uint32_t* u = reinterpret_cast<uint32_t*>(o);
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        u[e] = mes::pack_bf16x2(kv8::decode<kKind>(w[e >> 1] >> (16 * (e & 1))) * s,
+                                kv8::decode<kKind>(w[e >> 1] >> (16 * (e & 1) + 8)) * s);
+    }
+    out[2 * i] = o[0];
+    out[2 * i + 1] = o[1];
+  }
+}
+
+// ------------------------------------------ evict --------------------------------------
+// Selection: a cluster for each (sequence, head).  The candidates (all but the last `recent`
+// tokens) are cut into one contiguous slice a block, whose sums are turned into ordered integers
+// once, in shared memory where they fit.  The k-th largest follows from three histograms of 11,
+// 11 and 10 bits, added over the cluster through distributed shared memory; then each warp walks
+// its part of the slice in token order, so the kept indices come out sorted and a tie goes to
+// the lower index.
+constexpr int kSelThreads = 1024, kBins = 2048, kSelWarps = kSelThreads / 32;
+
+// Larger float -> larger integer; -0 equals +0 and NaN is lowest.
+__device__ __forceinline__ uint32_t order_key(float f) {
+  if (!(f == f)) return 0u;
+  const uint32_t u = __float_as_uint(f + 0.f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+struct SelShared {
+  uint32_t hist[kBins];
+  uint32_t warp_sum[2][kSelWarps];
+  uint32_t digit, above;       // this pass's bin and how many keys lie above it
+  uint32_t greater, equal;     // this block's counts against the threshold
+};
+
+__device__ __forceinline__ uint32_t ld_dsmem_u32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+
+__global__ void __launch_bounds__(kSelThreads)
+kv8_select_kernel(const float* __restrict__ sums, const int32_t* __restrict__ table, int64_t width,
+                  const int32_t* __restrict__ ctx, int Hkv, int P, int64_t num_pages, int keep,
+                  int recent, int cap, int ranks, int32_t* __restrict__ kept,
+                  int32_t* __restrict__ new_lens) {
+  extern __shared__ uint32_t cached[];
+  __shared__ SelShared sh;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int rank = ranks > 1 ? static_cast<int>(mes::cluster_ctarank()) : 0;
+  const int64_t item = blockIdx.x / ranks, b = item / Hkv;
+  const int h = static_cast<int>(item - b * Hkv);
+  int len = ctx[b];
+  if (len < 0 || len > width * P) {
+    if (tid == 0) record(MES_ERR_INVALID);
+    len = len < 0 ? 0 : static_cast<int>(width * P);
+  }
+  int32_t* out = kept + item * keep;
+  const int left = min(len, keep);
+  if (h == 0 && rank == 0 && tid == 0) new_lens[b] = left;
+  if (len <= keep) {   // nothing to evict (uniform over the cluster)
+    for (int i = rank * kSelThreads + tid; i < keep; i += ranks * kSelThreads) out[i] = i < len ? i : -1;
+    return;
+  }
+  const int n = len - recent;                       // candidates; recent <= keep < len
+  const uint32_t k = static_cast<uint32_t>(keep - recent);
+  for (int i = rank * kSelThreads + tid; i < recent; i += ranks * kSelThreads) out[k + i] = n + i;
+  if (k == 0) return;
+  // Slices are multiples of 32 tokens.
+  const int slice = ((n + ranks - 1) / ranks + 31) / 32 * 32;
+  const int lo = min(rank * slice, n), count = min(lo + slice, n) - lo;
+  auto load = [&](int i) {
+    const int t = lo + i;
+    int64_t page = table[b * width + t / P];
+    if (page < 0 || page >= num_pages) {
+      record(MES_ERR_INVALID);
+      page = 0;
+    }
+    return order_key(sums[(page * Hkv + h) * P + t % P]);
+  };
+  for (int i = tid; i < min(count, cap); i += kSelThreads) cached[i] = load(i);
+  auto key = [&](int i) { return i < cap ? cached[i] : load(i); };
+
+  uint32_t prefix = 0, want = k;      // the threshold's high bits; its place among the keys that share them
+  const int shifts[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = shifts[pass];
+    const uint32_t mask = (1u << bits[pass]) - 1, high = pass == 0 ? 0u : ~((1u << shifts[pass - 1]) - 1);
+    for (int i = tid; i < kBins; i += kSelThreads) sh.hist[i] = 0;
+    __syncthreads();
+    for (int i = tid; i < count; i += kSelThreads) {
+      const uint32_t x = key(i);
+      if ((x & high) == prefix) atomicAdd(&sh.hist[(x >> shift) & mask], 1u);
+    }
+    if (ranks > 1) mes::cluster_sync(); else __syncthreads();
+    // Bins from the top: thread t owns the pair of bins 2047 - 2t and 2046 - 2t.
+    const int top = kBins - 1 - 2 * tid;
+    uint32_t hi = 0, lo2 = 0;
+    if (ranks > 1) {
+      const uint32_t at = mes::smem_u32(&sh.hist[top - 1]);
+      for (int r = 0; r < ranks; ++r) {
+        const uint32_t a = mes::mapa_shared(at, r);
+        lo2 += ld_dsmem_u32(a);
+        hi += ld_dsmem_u32(a + 4);
+      }
+    } else {
+      hi = sh.hist[top];
+      lo2 = sh.hist[top - 1];
+    }
+    uint32_t x = hi + lo2;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) sh.warp_sum[0][warp] = x;
+    __syncthreads();
+    uint32_t before = 0;
+    for (int w = 0; w < warp; ++w) before += sh.warp_sum[0][w];
+    before += x - hi - lo2;          // keys in bins above this thread's
+    if (before < want && before + hi >= want) {
+      sh.digit = top;
+      sh.above = before;
+    } else if (before + hi < want && before + hi + lo2 >= want) {
+      sh.digit = top - 1;
+      sh.above = before + hi;
+    }
+    if (ranks > 1) mes::cluster_sync(); else __syncthreads();   // also: the histograms may be reused
+    prefix |= sh.digit << shift;
+    want -= sh.above;
+  }
+  // Keep every key above `prefix` and the first `want` equal to it.
+  const int per_warp = (slice / 32 + kSelWarps - 1) / kSelWarps * 32;
+  const int w0 = min(warp * per_warp, count), w1 = min(w0 + per_warp, count);
+  uint32_t gt = 0, eq = 0;
+  for (int i = w0 + lane; i < w1; i += 32) {
+    const uint32_t x = key(i);
+    gt += x > prefix;
+    eq += x == prefix;
+  }
+  gt = __reduce_add_sync(0xffffffffu, gt);
+  eq = __reduce_add_sync(0xffffffffu, eq);
+  if (lane == 0) {
+    sh.warp_sum[0][warp] = gt;
+    sh.warp_sum[1][warp] = eq;
+  }
+  __syncthreads();
+  if (tid == 0) {
+    uint32_t a = 0, e = 0;
+    for (int w = 0; w < kSelWarps; ++w) {
+      a += sh.warp_sum[0][w];
+      e += sh.warp_sum[1][w];
+    }
+    sh.greater = a;
+    sh.equal = e;
+  }
+  if (ranks > 1) mes::cluster_sync(); else __syncthreads();
+  uint32_t gt_before = 0, eq_before = 0;
+  for (int r = 0; r < rank; ++r) {
+    gt_before += ld_dsmem_u32(mes::mapa_shared(mes::smem_u32(&sh.greater), r));
+    eq_before += ld_dsmem_u32(mes::mapa_shared(mes::smem_u32(&sh.equal), r));
+  }
+  for (int w = 0; w < warp; ++w) {
+    gt_before += sh.warp_sum[0][w];
+    eq_before += sh.warp_sum[1][w];
+  }
+  for (int i0 = w0; i0 < w1; i0 += 32) {
+    const int i = i0 + lane;
+    const uint32_t x = i < w1 ? key(i) : 0u;
+    const uint32_t is_gt = __ballot_sync(0xffffffffu, i < w1 && x > prefix);
+    const uint32_t is_eq = __ballot_sync(0xffffffffu, i < w1 && x == prefix);
+    const uint32_t below = (1u << lane) - 1;
+    const uint32_t g = gt_before + __popc(is_gt & below), e = eq_before + __popc(is_eq & below);
+    if (i < w1 && (x > prefix || (x == prefix && e < want))) out[g + min(e, want)] = lo + i;
+    gt_before += __popc(is_gt);
+    eq_before += __popc(is_eq);
+  }
+  if (ranks > 1) mes::cluster_sync();    // no block leaves while another reads its counts
+}
+
+// Compaction: run (sequence, new page, side, head) gathers its tokens in kept order.  The run's
+// scale is the largest of its sources' scales, so tokens from the source that has it move
+// unchanged and the others are re-rounded once.
+template <int kKind, int P>
+__global__ void __launch_bounds__(Shape<P>::kThreads)
+kv8_compact_kernel(uint8_t* codes, float* scales, float* sums, const int32_t* __restrict__ table,
+                   int64_t width, const int32_t* __restrict__ new_table, int64_t new_width,
+                   const int32_t* __restrict__ kept, int keep, int Hkv, int64_t num_pages) {
+  __shared__ float red[8];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t b = blockIdx.x / new_width, j = blockIdx.x - b * new_width;
+  const int run = blockIdx.y * Shape<P>::kRuns + warp / Shape<P>::kRunWarps;
+  const int side = run >= Hkv, h = run - side * Hkv;
+  bool ok = run < 2 * Hkv;
+  int64_t to = 0;
+  if (ok) {
+    to = new_table[b * new_width + j];
+    if (to < 0 || to >= num_pages) {
+      ok = false;
+      record(MES_ERR_INVALID);
+    }
+  }
+  // Lane l < 16 looks up token l of the warp's 16 rows.
+  const int slot0 = warp % Shape<P>::kRunWarps * kWarpRows;
+  const int64_t place = j * P + slot0 + (lane & 15);
+  const int t = ok && place < keep ? kept[(b * Hkv + h) * keep + place] : -1;
+  int64_t row = -1;
+  float s = 0.f, sum = 0.f;
+  if (t >= 0) {
+    const int64_t page = table[b * width + t / P];
+    if (page < 0 || page >= num_pages) {
+      record(MES_ERR_INVALID);
+    } else {
+      const int64_t si = (page * 2 + side) * Hkv + h;
+      row = si * P + t % P;
+      s = scales[si];
+      if (side == 0) sum = sums[(page * Hkv + h) * P + t % P];
+    }
+  }
+  uint4 v[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int64_t r = __shfl_sync(0xffffffffu, row, 4 * i + (lane >> 3));
+    v[i] = r >= 0 ? *reinterpret_cast<const uint4*>(codes + r * kv8::kD + (lane & 7) * 16)
+                  : make_uint4(0, 0, 0, 0);
+  }
+  const float now = run_max<P>(s, red), safe = now > 0.f ? now : 1.f;
+  const int64_t di = (to * 2 + side) * Hkv + h;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float was = __shfl_sync(0xffffffffu, s, 4 * i + (lane >> 3));
+    if (was != now) {
+      uint32_t* w = reinterpret_cast<uint32_t*>(&v[i]);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t o = 0;
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          o |= kv8::encode<kKind>(kv8::decode<kKind>(w[e] >> (8 * q)) * was / safe) << (8 * q);
+        w[e] = o;
+      }
+    }
+    if (ok)
+      *reinterpret_cast<uint4*>(codes + (di * P + slot0 + 4 * i + (lane >> 3)) * kv8::kD + (lane & 7) * 16) = v[i];
+  }
+  if (!ok) return;
+  if (side == 0 && lane < 16) sums[(to * Hkv + h) * P + slot0 + lane] = sum;
+  if (lane == 0 && warp % Shape<P>::kRunWarps == 0) scales[di] = now;
+}
+
+template <typename F>
+int by_page(int page, F f) {
+  switch (page) {
+    case 16: return f(std::integral_constant<int, 16>());
+    case 32: return f(std::integral_constant<int, 32>());
+    case 64: return f(std::integral_constant<int, 64>());
+    default: return f(std::integral_constant<int, 128>());
+  }
+}
+
+unsigned run_blocks(int Hkv, int runs) { return (unsigned)((2 * Hkv + runs - 1) / runs); }
+
+}  // namespace
+
+extern "C" int mes_kv8_cache_take_error(int* code) {
+  int v = 0, zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbol(&v, g_err_kv8_cache, sizeof(int));
+  if (e != cudaSuccess) return MES_ERR_CUDA;
+  e = cudaMemcpyToSymbol(g_err_kv8_cache, &zero, sizeof(int));
+  *code = v;
+  return mes_host::from_cuda(e);
+}
+
+extern "C" int mes_kv8_append(int dtype, const void* K, int64_t ldk, const void* V, int64_t ldv,
+                              void* codes, float* scales, float* sums, const int32_t* block_table,
+                              int64_t table_width, const int32_t* cu_new, const int32_t* context_lens,
+                              int64_t B, int64_t T, int64_t max_new, int Hkv, int D, int page_size,
+                              int64_t num_pages, void* stream) {
+  if (!kv8::valid_cache(dtype, num_pages, Hkv, D, page_size)) return MES_ERR_INVALID;
+  if (B < 0 || T < 0 || max_new < 0 || max_new > T || table_width <= 0) return MES_ERR_INVALID;
+  if (table_width > 0x7fffffffll / page_size || T > 0x7fffffffll) return MES_ERR_INVALID;
+  if (ldk < (int64_t)Hkv * D || ldv < (int64_t)Hkv * D || ldk % 8 || ldv % 8) return MES_ERR_INVALID;
+  if (B == 0 || T == 0 || max_new == 0) return MES_OK;
+  if (!K || !V || !codes || !scales || !block_table || !cu_new || !context_lens) return MES_ERR_INVALID;
+  if (!kv8::aligned(K, 16) || !kv8::aligned(V, 16) || !kv8::aligned(codes, 16) || !kv8::aligned(scales, 4) ||
+      !kv8::aligned(sums, 4) || !kv8::aligned(block_table, 4) || !kv8::aligned(cu_new, 4) ||
+      !kv8::aligned(context_lens, 4))
+    return MES_ERR_ALIGN;
+  // Pages that max_new tokens can touch, starting anywhere in one.
+  const int64_t pages = (max_new + page_size - 2) / page_size + 1;
+  if (B * pages > 0x7fffffffll) return MES_ERR_INVALID;
+  return by_page(page_size, [&](auto p) {
+    constexpr int P = decltype(p)::value;
+    const dim3 grid((unsigned)(B * pages), run_blocks(Hkv, Shape<P>::kRuns));
+    auto kernel = dtype == kv8::kInt8 ? kv8_append_kernel<kv8::kInt8, P> : kv8_append_kernel<kv8::kE4m3, P>;
+    kernel<<<grid, Shape<P>::kThreads, 0, (cudaStream_t)stream>>>(
+        (const __nv_bfloat16*)K, ldk, (const __nv_bfloat16*)V, ldv, (uint8_t*)codes, scales, sums,
+        block_table, table_width, cu_new, context_lens, T, (int)pages, Hkv, num_pages);
+    return mes_host::from_cuda(cudaGetLastError());
+  });
+}
+
+extern "C" int mes_kv8_read(int dtype, const void* codes, const float* scales, const int32_t* pages,
+                            int64_t n, int Hkv, int D, int page_size, int64_t num_pages, void* out,
+                            void* stream) {
+  if (!kv8::valid_cache(dtype, num_pages, Hkv, D, page_size) || n < 0) return MES_ERR_INVALID;
+  if (n == 0) return MES_OK;
+  if (!codes || !scales || !pages || !out) return MES_ERR_INVALID;
+  if (!kv8::aligned(codes, 16) || !kv8::aligned(out, 16) || !kv8::aligned(scales, 4) || !kv8::aligned(pages, 4))
+    return MES_ERR_ALIGN;
+  const int64_t run_chunks = (int64_t)page_size * D / 16, page_chunks = run_chunks * 2 * Hkv;
+  if (n > 0x7fffffffffffffffll / (page_chunks * 32)) return MES_ERR_INVALID;
+  const int64_t chunks = n * page_chunks, cap = (int64_t)mes_host::sm_count() * 32;
+  const int64_t blocks = (chunks + 255) / 256;
+  auto kernel = dtype == kv8::kInt8 ? kv8_read_kernel<kv8::kInt8> : kv8_read_kernel<kv8::kE4m3>;
+  kernel<<<(unsigned)(blocks < cap ? blocks : cap), 256, 0, (cudaStream_t)stream>>>(
+      (const uint8_t*)codes, scales, pages, chunks, page_chunks, run_chunks, num_pages, (uint4*)out);
+  return mes_host::from_cuda(cudaGetLastError());
+}
+
+extern "C" int mes_kv8_evict(int dtype, void* codes, float* scales, float* sums,
+                             const int32_t* block_table, int64_t table_width,
+                             const int32_t* context_lens, int64_t B, const int32_t* new_table,
+                             int64_t new_width, int64_t keep, int64_t recent, int Hkv, int D,
+                             int page_size, int64_t num_pages, int32_t* kept, int32_t* new_lens,
+                             void* stream) {
+  if (!kv8::valid_cache(dtype, num_pages, Hkv, D, page_size)) return MES_ERR_INVALID;
+  if (B < 0 || table_width <= 0 || keep <= 0 || recent < 0 || recent > keep) return MES_ERR_INVALID;
+  if (table_width > 0x7fffffffll / page_size || keep > 0x7fffffffll - 128) return MES_ERR_INVALID;
+  if (new_width != (keep + page_size - 1) / page_size) return MES_ERR_INVALID;
+  if (B == 0) return MES_OK;
+  if (!codes || !scales || !sums || !block_table || !context_lens || !new_table || !kept || !new_lens)
+    return MES_ERR_INVALID;
+  if (!kv8::aligned(codes, 16) || !kv8::aligned(scales, 4) || !kv8::aligned(sums, 4) ||
+      !kv8::aligned(block_table, 4) || !kv8::aligned(context_lens, 4) || !kv8::aligned(new_table, 4) ||
+      !kv8::aligned(kept, 4) || !kv8::aligned(new_lens, 4))
+    return MES_ERR_ALIGN;
+  // Blocks of a cluster: one for each 4096 possible tokens, at most 8 (the portable limit).
+  const int64_t most = table_width * page_size;
+  int ranks = 1;
+  while (ranks < 8 && (int64_t)ranks * 4096 < most) ranks *= 2;
+  if (B * Hkv > 0x7fffffffll / ranks || B * new_width > 0x7fffffffll) return MES_ERR_INVALID;
+  // Keys kept in shared memory (up to 192 KB); a longer slice's rest is read again in each pass.
+  const int64_t slice = (most + ranks - 1) / ranks + 32;
+  const int cap = (int)(slice < 49152 ? slice : 49152);
+  static std::atomic<uint64_t> configured{0};
+  int st = mes_host::once_per_device(configured, [] {
+    return mes_host::from_cuda(cudaFuncSetAttribute(
+        kv8_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 49152 * 4));
+  });
+  if (st != MES_OK) return st;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(B * Hkv * ranks));
+  cfg.blockDim = dim3(kSelThreads);
+  cfg.dynamicSmemBytes = (size_t)cap * 4;
+  cfg.stream = (cudaStream_t)stream;
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = ranks;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  cudaError_t e = cudaLaunchKernelEx(&cfg, kv8_select_kernel, (const float*)sums, block_table, table_width,
+                                     context_lens, Hkv, page_size, num_pages, (int)keep, (int)recent,
+                                     cap, ranks, kept, new_lens);
+  if (e != cudaSuccess) return MES_ERR_CUDA;
+  return by_page(page_size, [&](auto p) {
+    constexpr int P = decltype(p)::value;
+    const dim3 grid((unsigned)(B * new_width), run_blocks(Hkv, Shape<P>::kRuns));
+    auto kernel = dtype == kv8::kInt8 ? kv8_compact_kernel<kv8::kInt8, P> : kv8_compact_kernel<kv8::kE4m3, P>;
+    kernel<<<grid, Shape<P>::kThreads, 0, (cudaStream_t)stream>>>(
+        (uint8_t*)codes, scales, sums, block_table, table_width, new_table, new_width, kept, (int)keep,
+        Hkv, num_pages);
+    return mes_host::from_cuda(cudaGetLastError());
+  });
+}
