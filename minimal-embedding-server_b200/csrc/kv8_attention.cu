@@ -222,8 +222,7 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
       row[half] = (int)(run * p.P + (t & (p.P - 1)));
       ks[half] = p.scales[run];
       vs[half] = p.scales[run + p.Hkv];
-      // A page of zeros has scale 0: any factor will do for its V codes.
-      if (!(vs[half] > 0.f)) vs[half] = 1.f;
+      if (vs[half] == 0.f) vs[half] = -1.f;      // marks V values that are all 0
       ++t_halves;
     }
     t_row0 = row[0];
@@ -344,7 +343,13 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
         phase ^= 1u << stage;
         const uint8_t* kt = sh.ring[warp][stage];
         const uint8_t* vt = kt + kHalfBytes;
-        const float4 sc = sh.sc[warp][stage];
+        float4 sc = sh.sc[warp][stage];
+        // V codes of scale 0 count as 0 (their factor is then free, here 1); so do slots past the
+        // end, which hold anything, NaN codes too, and 0 * NaN is NaN.
+        const int v_end[2] = {sc.z < 0.f ? 0 : s.len, sc.w < 0.f ? 0 : s.len};
+        const bool tail = t0 + kTile > min(v_end[0], v_end[1]);
+        sc.z = fabsf(sc.z);
+        sc.w = fabsf(sc.w);
         // ---- S = Q K^T ----
         float S[R][4][4];
 #pragma unroll
@@ -443,7 +448,6 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
             P[r][j] = make_uint4(pw[2 * j][0], pw[2 * j][1], pw[2 * j + 1][0], pw[2 * j + 1][1]);
         }
         // ---- O += P V ----
-        const bool tail = t0 + kTile > s.len;
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           uint4 v[4];
@@ -451,8 +455,7 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
           for (int e = 0; e < 4; ++e) {
             const int key = 8 * (2 * j + (e >> 1)) + key_of(2 * c + (e & 1));
             v[e] = *reinterpret_cast<const uint4*>(vt + key * kv8::kD + ((g ^ (key & 7)) << 4));
-            // Slots past the end hold anything, NaN codes too, and 0 * NaN is NaN.
-            if (tail && t0 + key >= s.len) v[e] = make_uint4(0, 0, 0, 0);
+            if (tail && t0 + key >= v_end[j]) v[e] = make_uint4(0, 0, 0, 0);
           }
 #pragma unroll
           for (int q = 0; q < 4; ++q) {
