@@ -13,16 +13,17 @@
 //
 // A block is four warps.  Each takes 32 keys of a unit for itself: its own ring of TMA tiles
 // (128-byte swizzle, so the 16-byte reads below meet no bank conflict), its own running maximum
-// and sum.  Codes become f16 in registers (exact for both types) and feed mma.sync with the query
-// rows as the 16-row operand; with so few rows a tcgen05 tile of 128 rows would be mostly empty
-// and its operands would have to be converted and written back to shared memory first.
+// and sum.  Codes become f16 in registers (exact for both types) and feed mma.sync in the
+// transposed form, S^T = K Q^T and O^T = V^T P^T: keys, then head dimensions, are the 16-row
+// operand and 8 query rows the columns, so that a token step's 1 to 8 rows fill a product.  A
+// tcgen05 tile would have the converted codes written back to shared memory first.
 //
-// The order of the contracted index is free, so a lane's 16-byte chunk of a K row is its B fragment
+// The order of the contracted index is free, so a lane's 16-byte chunk of a K row is its A fragment
 // for four steps, and four lanes' V rows are transposed with byte permutes.
 //
 // Scales: a page's K scale multiplies its logits.  Its V scale vs goes into the exponent,
-// p' = exp2(s + log2(vs) - m), with m the running maximum of s + log2(vs): p' stays within f16
-// whatever the scales are, and the softmax sum adds p' / vs.
+// p' = exp2(s + log2(vs) - m), with m a running reference near the maximum of s + log2(vs): p'
+// stays within f16 whatever the scales are, and the softmax sum adds p' / vs.
 #include "kv8.cuh"
 
 namespace {
@@ -34,25 +35,33 @@ constexpr int kStages = 2;
 constexpr int kMaxSeqs = 1024;
 constexpr int kHalfBytes = kTile * kv8::kD;                 // one side of a stage
 constexpr int kStageBytes = 2 * kHalfBytes;
-constexpr int kORow = 144;        // floats of an output row in shared memory (bank spread)
-constexpr float kShift = 10.f;    // p' is held times 2^10: f16 keeps weights down to 2^-24 of the largest
-// Blocks of an SM that shared memory holds.
-constexpr int blocks_per_sm(int R) { return R == 1 ? 2 : 1; }
+// p' is 2^kShift for a tile's largest value when its reference is set, and may grow to 2^kMost: f16
+// keeps weights down to 2^-24 of that largest one and ends at 2^16.
+constexpr float kShift = 10.f, kMost = 15.f;
+// Blocks of an SM: registers and shared memory hold three with 8 query rows, two with more.
+constexpr int blocks_per_sm(int N) { return N == 1 ? 3 : 2; }
 
-template <int R>
+// N: 8-row tiles of query rows.
+template <int N>
 struct Smem {
   uint8_t ring[kWarps][kStages][kStageBytes];   // 1024-byte aligned
-  float o[kWarps][16 * R][kORow];
-  uint4 q[R][8][32];                            // A fragments
-  float m[kWarps][16 * R], l[kWarps][16 * R];
-  float qscale[16 * R];                         // logit factor of a row, in the exp2 domain
-  int last[16 * R];                             // last visible key of a row
-  float4 sc[kWarps][kStages];                   // K and V scale factors of a tile's two halves
+  union {
+    float4 o[2][N][8][32];                      // two warps' results on their way to the others
+    uint2 q1[8][32];                            // N == 1: Q fragments on their way to registers
+  };
+  uint2 q[N == 1 ? 1 : N][8][32];               // N > 1: Q fragments
+  float2 ml[2][8 * N];                          // reference and sum of the rows of `o`
+  float qscale[8 * N];                          // logit factor of a row, in the exp2 domain
+  int last[8 * N];                              // last visible key of a row
+  float2 sc[kWarps][kStages][3];                // factors of a tile's two halves: K scale, log2 and
+                                                // reciprocal of the V scale (-1: V values all 0)
   uint64_t full[kWarps][kStages];
-  int prefix[kMaxSeqs + 1];
   int warp_sum[kWarps];
   int abort;
+  int prefix[1];                                // [B + 1]
 };
+template <int N>
+constexpr size_t smem_bytes(int B) { return sizeof(Smem<N>) + 4 * (size_t)B; }
 
 struct Params {
   const __nv_bfloat16* q;
@@ -66,27 +75,36 @@ struct Params {
   int64_t num_pages;
   float scale;
   __nv_bfloat16* out;
-  int* prefix_out;      // [B + 1] for the join
-  float* part_o;        // [blocks][2][16 R][128]
-  float2* part_ml;      // [blocks][2][16 R]
+  float* part_o;        // [blocks][2][8 N][128]
+  float2* part_ml;      // [blocks][2][8 N]
   float* lse;           // [T * Hq] with sums, else null
   float* logits;        // [T * Hq][max_ctx] with sums, else null
   int64_t max_ctx;
 };
 
-// Row p of a tile's 8-key group that lane group n (or column n) holds: rows n and n ^ 1 differ in
-// bit 2, and for a fixed parity the rows of n / 2 = 0..3 differ in bits 1 and 2, which is what the
-// swizzled K and V reads need to touch every bank once.
+// Key of an 8-key group that is row n of a product: keys of n and n ^ 1 differ in bit 2, and for a
+// fixed parity the keys of n / 2 = 0..3 differ in bits 1 and 2, which is what the swizzled K and V
+// reads need to touch every bank once.
 __device__ __forceinline__ int key_of(int n) {
   return ((n >> 1) & 1) | (((n >> 2) & 1) << 1) | (((n ^ (n >> 1)) & 1) << 2);
 }
 
-__device__ __forceinline__ void mma_f16(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                        uint32_t b0, uint32_t b1) {
   asm volatile(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-      : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Transposes an 8 x 8 matrix of 16-bit values: lane (g, c) gives row g, columns 2c and 2c + 1.
+__device__ __forceinline__ uint32_t transpose8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
+  return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
 }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -99,7 +117,8 @@ __device__ __forceinline__ float ex2(float x) {
 // flipped, is the low mantissa of 1024, and 1024 + 128 is taken off again.  e4m3: bytes (0, 1) and
 // (2, 3) by the conversion instruction.
 __device__ __forceinline__ uint32_t int8_pair(uint32_t w) {
-  const uint32_t v = (w & 0x00ff00ffu) ^ 0x64806480u;
+  uint32_t v;      // (w & 0x00ff00ff) ^ 0x64806480
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(v) : "r"(w), "r"(0x00ff00ffu), "r"(0x64806480u));
   const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&v), __half2half2(__ushort_as_half(0x6480)));
   return *reinterpret_cast<const uint32_t*>(&r);
 }
@@ -117,8 +136,8 @@ __device__ __forceinline__ void convert(uint32_t w, uint32_t& a, uint32_t& b) {
 // Units of a sequence's items and their number.  A sequence with query rows has at least one unit
 // an item, so that rows that see nothing are written too.
 __device__ __forceinline__ int units_of(int len) { return len > 0 ? (len + kUnit - 1) / kUnit : 1; }
-template <int R>
-__device__ __forceinline__ int row_tiles(int n, int G) { return (n * G + 16 * R - 1) / (16 * R); }
+template <int N>
+__device__ __forceinline__ int row_tiles(int n, int G) { return (n * G + 8 * N - 1) / (8 * N); }
 
 struct Seq {
   int r0, n, len;
@@ -139,14 +158,18 @@ __device__ __forceinline__ Seq sequence(const Params& p, int b) {
 // First unit of block i's share.
 __device__ __forceinline__ int share(int64_t units, int i, int blocks) { return (int)(units * i / blocks); }
 
-template <int kKind, int R, bool kSums>
-__global__ void __launch_bounds__(kThreads, blocks_per_sm(R))
+template <int kKind, int N, bool kSums>
+__global__ void __launch_bounds__(kThreads, blocks_per_sm(N))
 kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
-  extern __shared__ uint8_t raw[];
-  Smem<R>& sh = *reinterpret_cast<Smem<R>*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
-  constexpr int kRows = 16 * R;
+  extern __shared__ __align__(1024) uint8_t raw[];
+  Smem<N>& sh = *reinterpret_cast<Smem<N>*>(raw);
+  constexpr int kRows = 8 * N;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
 
+  if (mes::smem_u32(raw) & 1023) {      // the swizzle goes by the address
+    if (tid == 0) atomicCAS(&g_err_kv8_attention, 0, MES_ERR_ALIGN);
+    return;
+  }
   if (tid == 0) {
     sh.abort = 0;
     for (int w = 0; w < kWarps; ++w)
@@ -154,6 +177,8 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
     mes::fence_barrier_init();
     mes::tma_prefetch_desc(&map);
   }
+  // The join may be launched as soon as every block of this grid runs (it waits for their end).
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   // Units before each sequence.
   int total = 0;
   for (int b0 = 0; b0 < p.B; b0 += kThreads) {
@@ -161,7 +186,7 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
     int x = 0;
     if (b < p.B) {
       const Seq s = sequence(p, b);
-      x = s.n > 0 ? units_of(s.len) * p.Hkv * row_tiles<R>(s.n, p.G) : 0;
+      x = s.n > 0 ? units_of(s.len) * p.Hkv * row_tiles<N>(s.n, p.G) : 0;
     }
     const int mine = x;
 #pragma unroll
@@ -179,8 +204,6 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
   }
   if (tid == 0) sh.prefix[p.B] = total;
   __syncthreads();
-  if (blockIdx.x == 0)
-    for (int b = tid; b <= p.B; b += kThreads) p.prefix_out[b] = sh.prefix[b];
   const int blocks = min((int)gridDim.x, total);
   if ((int)blockIdx.x >= blocks) return;
   const int first = share(total, blockIdx.x, blocks), end = share(total, blockIdx.x + 1, blocks);
@@ -197,61 +220,76 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
   // ---- the warp's tiles: unit first + i is its tile i ----
   // Lane j holds what tiles 32 i + j need: the cache rows of its halves and its scales.
   int t_row0 = 0, t_row1 = 0, t_halves = 0;
-  float4 t_sc = make_float4(0.f, 0.f, 0.f, 0.f);
+  float2 t_ks = make_float2(0.f, 0.f), t_vs = make_float2(1.f, 1.f), t_lv = t_ks, t_iv = t_ks;
   auto look_up = [&](int i0) {
     const int u = first + i0 + lane;
     t_halves = 0;
+    t_ks = make_float2(0.f, 0.f);
+    t_vs = make_float2(1.f, 1.f);
     if (u >= end) return;
     const int b = find(u);
     const Seq s = sequence(p, b);
     const int units = units_of(s.len), rest = u - sh.prefix[b], item = rest / units;
     const int t0 = (rest - item * units) * kUnit + warp * kTile;
-    const int h = item / row_tiles<R>(s.n, p.G);
-    float ks[2] = {0.f, 0.f}, vs[2] = {1.f, 1.f};
-    int row[2] = {0, 0};
+    const int h = item / row_tiles<N>(s.n, p.G);
+    int64_t page[2] = {0, 0};
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+      if (t0 + 16 * half < s.len) {
+        page[half] = p.table[(int64_t)b * p.width + ((t0 + 16 * half) >> p.page_shift)];
+        ++t_halves;
+      }
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      const int t = t0 + 16 * half;
-      if (t >= s.len) continue;
-      int64_t page = p.table[(int64_t)b * p.width + (t >> p.page_shift)];
-      if (page < 0 || page >= p.num_pages) {
+      if (page[half] < 0 || page[half] >= p.num_pages) {
         atomicCAS(&g_err_kv8_attention, 0, MES_ERR_INVALID);
-        page = 0;
+        page[half] = 0;
       }
-      const int64_t run = page * 2 * p.Hkv + h;
-      row[half] = (int)(run * p.P + (t & (p.P - 1)));
-      ks[half] = p.scales[run];
-      vs[half] = p.scales[run + p.Hkv];
-      if (vs[half] == 0.f) vs[half] = -1.f;      // marks V values that are all 0
-      ++t_halves;
+      page[half] = page[half] * 2 * p.Hkv + h;       // the run of K; that of V is Hkv further
     }
-    t_row0 = row[0];
-    t_row1 = row[1];
-    t_sc = make_float4(ks[0], ks[1], vs[0], vs[1]);
+    t_row0 = (int)(page[0] * p.P + (t0 & (p.P - 1)));
+    t_row1 = (int)(page[1] * p.P + ((t0 + 16) & (p.P - 1)));
+    if (t_halves > 0) {
+      t_ks.x = p.scales[page[0]];
+      t_vs.x = p.scales[page[0] + p.Hkv];
+    }
+    if (t_halves > 1) {
+      t_ks.y = p.scales[page[1]];
+      t_vs.y = p.scales[page[1] + p.Hkv];
+    }
   };
-  auto issue = [&](int i) {      // the whole warp; tile i into stage i % kStages
-    if (first + i >= end) return;
-    if ((i & 31) == 0) look_up(i);
-    const int src = i & 31, stage = i % kStages;
-    const int halves = __shfl_sync(0xffffffffu, t_halves, src);
-    const int row0 = __shfl_sync(0xffffffffu, t_row0, src), row1 = __shfl_sync(0xffffffffu, t_row1, src);
-    if (lane == src) sh.sc[warp][stage] = t_sc;
-    if (halves == 0 || lane != 0) return;
-    uint64_t* bar = &sh.full[warp][stage];
-    uint8_t* k = sh.ring[warp][stage];
+  auto load = [&](int i) {       // one lane: tile i's copies into stage i % kStages
+    uint64_t* bar = &sh.full[warp][i % kStages];
+    uint8_t* k = sh.ring[warp][i % kStages];
     const int vrow = p.Hkv << p.page_shift;
     if (p.P >= kTile) {       // one box of 32 rows a side
       mes::mbar_arrive_expect_tx(bar, kStageBytes);
-      mes::tma_load_2d(k, &map, bar, 0, row0);
-      mes::tma_load_2d(k + kHalfBytes, &map, bar, 0, row0 + vrow);
+      mes::tma_load_2d(k, &map, bar, 0, t_row0);
+      mes::tma_load_2d(k + kHalfBytes, &map, bar, 0, t_row0 + vrow);
     } else {                  // pages of 16: a box for each half that holds tokens
-      mes::mbar_arrive_expect_tx(bar, halves * (kStageBytes / 2));
-      mes::tma_load_2d(k, &map, bar, 0, row0);
-      mes::tma_load_2d(k + kHalfBytes, &map, bar, 0, row0 + vrow);
-      if (halves == 2) {
-        mes::tma_load_2d(k + kHalfBytes / 2, &map, bar, 0, row1);
-        mes::tma_load_2d(k + kHalfBytes + kHalfBytes / 2, &map, bar, 0, row1 + vrow);
+      mes::mbar_arrive_expect_tx(bar, t_halves * (kStageBytes / 2));
+      mes::tma_load_2d(k, &map, bar, 0, t_row0);
+      mes::tma_load_2d(k + kHalfBytes, &map, bar, 0, t_row0 + vrow);
+      if (t_halves == 2) {
+        mes::tma_load_2d(k + kHalfBytes / 2, &map, bar, 0, t_row1);
+        mes::tma_load_2d(k + kHalfBytes + kHalfBytes / 2, &map, bar, 0, t_row1 + vrow);
       }
+    }
+  };
+  auto issue = [&](int i) {      // the whole warp: tile i
+    if (first + i >= end) return;
+    const bool mine = lane == (i & 31);
+    if ((i & 31) == 0) look_up(i);
+    if (mine && t_halves > 0) load(i);
+    if ((i & 31) == 0) {         // the scales arrive behind the first copy
+      // V codes of scale 0 count as 0, so their factor is free, here 1; the mark is a reciprocal of -1.
+      t_lv = make_float2(t_vs.x == 0.f ? 0.f : log2f(t_vs.x), t_vs.y == 0.f ? 0.f : log2f(t_vs.y));
+      t_iv = make_float2(t_vs.x == 0.f ? -1.f : 1.f / t_vs.x, t_vs.y == 0.f ? -1.f : 1.f / t_vs.y);
+    }
+    if (mine) {
+      sh.sc[warp][i % kStages][0] = t_ks;
+      sh.sc[warp][i % kStages][1] = t_lv;
+      sh.sc[warp][i % kStages][2] = t_iv;
     }
   };
   for (int i = 0; i < kStages; ++i) issue(i);
@@ -262,7 +300,7 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
     // ---- segment: units [u, stop) of one item ----
     const int b = find(u);
     const Seq s = sequence(p, b);
-    const int units = units_of(s.len), tiles = row_tiles<R>(s.n, p.G);
+    const int units = units_of(s.len), tiles = row_tiles<N>(s.n, p.G);
     const int rest = u - sh.prefix[b], item = rest / units, unit0 = rest - item * units;
     const int h = item / tiles, tile = item - h * tiles;
     const int item0 = u - unit0, stop = min(end, item0 + units);
@@ -298,40 +336,45 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
       const int ex = min(max((int)((__float_as_uint(amax) >> 23) & 255) - 127, -110), 120);
       const float down = __uint_as_float((uint32_t)(127 + 8 - ex) << 23), up = __uint_as_float((uint32_t)(127 - 8 + ex) << 23);
       if (part == 0) sh.qscale[r] = p.scale * 1.4426950408889634f * up;
-      const int cc = part & 3, u0 = (part >> 2) * 4, fl = (r & 7) * 4 + cc, hi = (r >> 3) & 1;
+      const int cc = part & 3, u0 = (part >> 2) * 4, fl = (r & 7) * 4 + cc;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const float e0 = f[4 * w] * down, e1 = f[4 * w + 1] * down, e2 = f[4 * w + 2] * down, e3 = f[4 * w + 3] * down;
         const __half2 lo2 = kKind == kv8::kInt8 ? __floats2half2_rn(e0, e2) : __floats2half2_rn(e0, e1);
         const __half2 hi2 = kKind == kv8::kInt8 ? __floats2half2_rn(e1, e3) : __floats2half2_rn(e2, e3);
-        uint32_t* frag = reinterpret_cast<uint32_t*>(&sh.q[r >> 4][u0 + w][fl]);
-        frag[hi] = *reinterpret_cast<const uint32_t*>(&lo2);
-        frag[2 + hi] = *reinterpret_cast<const uint32_t*>(&hi2);
+        uint2* frag = N == 1 ? &sh.q1[u0 + w][fl] : &sh.q[r >> 3][u0 + w][fl];
+        *frag = make_uint2(*reinterpret_cast<const uint32_t*>(&lo2), *reinterpret_cast<const uint32_t*>(&hi2));
       }
     }
     __syncthreads();
-    float qs[R][2];
-    int last[R][2];
-    int first_last = 0x7fffffff;      // keys every row of this lane sees
+    // This lane's rows are 8 t + 2 c + e of tile t.
+    float qs[N][2];
+    int last[N][2];
+    int first_last = 0x7fffffff;      // keys that every row sees
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int t = 0; t < N; ++t)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        qs[r][e] = sh.qscale[16 * r + 8 * e + g];
-        last[r][e] = min(sh.last[16 * r + 8 * e + g], s.len - 1);
-        first_last = min(first_last, last[r][e]);
+        qs[t][e] = sh.qscale[8 * t + 2 * c + e];
+        last[t][e] = min(sh.last[8 * t + 2 * c + e], s.len - 1);
+        first_last = min(first_last, last[t][e]);
       }
     first_last = __reduce_min_sync(0xffffffffu, first_last);
+    uint2 q1[8];
+    if (N == 1) {
+#pragma unroll
+      for (int st = 0; st < 8; ++st) q1[st] = sh.q1[st][lane];
+    }
 
-    float O[R][16][4], m[R][2], l[R][2];
+    float O[N][8][4], m[N][2], l[N][2];
 #pragma unroll
-    for (int r = 0; r < R; ++r) {
+    for (int t = 0; t < N; ++t) {
 #pragma unroll
-      for (int t = 0; t < 16; ++t)
+      for (int d = 0; d < 8; ++d)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) O[r][t][e] = 0.f;
-      m[r][0] = m[r][1] = -INFINITY;
-      l[r][0] = l[r][1] = 0.f;
+        for (int e = 0; e < 4; ++e) O[t][d][e] = 0.f;
+      m[t][0] = m[t][1] = -INFINITY;
+      l[t][0] = l[t][1] = 0.f;
     }
 
     for (; u < stop; ++u) {
@@ -343,111 +386,131 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
         phase ^= 1u << stage;
         const uint8_t* kt = sh.ring[warp][stage];
         const uint8_t* vt = kt + kHalfBytes;
-        float4 sc = sh.sc[warp][stage];
-        // V codes of scale 0 count as 0 (their factor is then free, here 1); so do slots past the
-        // end, which hold anything, NaN codes too, and 0 * NaN is NaN.
-        const int v_end[2] = {sc.z < 0.f ? 0 : s.len, sc.w < 0.f ? 0 : s.len};
-        const bool tail = t0 + kTile > min(v_end[0], v_end[1]);
-        sc.z = fabsf(sc.z);
-        sc.w = fabsf(sc.w);
-        // ---- S = Q K^T ----
-        float S[R][4][4];
+        const float2 ks = sh.sc[warp][stage][0], lv = sh.sc[warp][stage][1], iv = sh.sc[warp][stage][2];
+        if (t0 + kTile > s.len || iv.x < 0.f || iv.y < 0.f) {
+          // V slots past the end hold anything, NaN codes too, and 0 * NaN is NaN; codes of scale 0
+          // count as 0.  Lane = slot.
+          if (t0 + lane >= s.len || (lane < 16 ? iv.x : iv.y) < 0.f) {
+            uint4* row = reinterpret_cast<uint4*>(const_cast<uint8_t*>(vt) + lane * kv8::kD);
 #pragma unroll
-        for (int r = 0; r < R; ++r)
+            for (int j = 0; j < 8; ++j) row[j] = make_uint4(0, 0, 0, 0);
+          }
+          mes::fence_proxy_async_smem();      // before the stage is loaded again
+          __syncwarp();
+        }
+        // ---- S^T = K Q^T: keys 16 mt + key_of(g) and 8 more by rows 2 c and 2 c + 1 ----
+        float S[N][2][4];
 #pragma unroll
-          for (int nt = 0; nt < 4; ++nt)
+        for (int t = 0; t < N; ++t)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) S[r][nt][e] = 0.f;
-        uint4 kw[4][2];
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) S[t][mt][e] = 0.f;
         const int kg = key_of(g);
 #pragma unroll
-        for (int nt = 0; nt < 4; ++nt)
-#pragma unroll
-          for (int half = 0; half < 2; ++half)
-            kw[nt][half] = *reinterpret_cast<const uint4*>(kt + (8 * nt + kg) * kv8::kD + (((c + 4 * half) ^ kg) << 4));
-#pragma unroll
-        for (int st = 0; st < 8; ++st) {
-          uint4 a[R];
-#pragma unroll
-          for (int r = 0; r < R; ++r) a[r] = sh.q[r][st][lane];
-#pragma unroll
-          for (int nt = 0; nt < 4; ++nt) {
-            const uint4& v = kw[nt][st >> 2];
-            const uint32_t w = (st & 3) == 0 ? v.x : (st & 3) == 1 ? v.y : (st & 3) == 2 ? v.z : v.w;
-            uint32_t b0, b1;
-            convert<kKind>(w, b0, b1);
-#pragma unroll
-            for (int r = 0; r < R; ++r) mma_f16(S[r][nt], a[r], b0, b1);
-          }
-        }
-        // ---- logits, running maximum ----
-        const float lv[2] = {__log2f(sc.z), __log2f(sc.w)};
-        const bool masked = t0 + kTile - 1 > first_last;
-        uint4 P[R][2];
-#pragma unroll
-        for (int r = 0; r < R; ++r) {
-          float mx[2] = {-INFINITY, -INFINITY};
+        for (int half = 0; half < 2; ++half) {
+          uint4 kw[4];
 #pragma unroll
           for (int nt = 0; nt < 4; ++nt)
+            kw[nt] = *reinterpret_cast<const uint4*>(kt + (8 * nt + kg) * kv8::kD + (((c + 4 * half) ^ kg) << 4));
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              const float ks = nt < 2 ? sc.x : sc.y;
-              float x = S[r][nt][e] * (ks * qs[r][e >> 1]);
-              if (masked) x = t0 + 8 * nt + key_of(2 * c + (e & 1)) > last[r][e >> 1] ? -INFINITY : x;
-              if (kSums) {
-                const int row = 16 * r + 8 * (e >> 1) + g, t = t0 + 8 * nt + key_of(2 * c + (e & 1));
-                if (row < rows && t < s.len) {
+          for (int st = 0; st < 4; ++st) {
+            uint2 b[N];
+#pragma unroll
+            for (int t = 0; t < N; ++t) b[t] = N == 1 ? q1[4 * half + st] : sh.q[t][4 * half + st][lane];
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt) {
+              uint32_t a0, a1, a2, a3;
+              convert<kKind>(word_of(kw[2 * mt], st), a0, a2);
+              convert<kKind>(word_of(kw[2 * mt + 1], st), a1, a3);
+#pragma unroll
+              for (int t = 0; t < N; ++t) mma_f16(S[t][mt], a0, a1, a2, a3, b[t].x, b[t].y);
+            }
+          }
+        }
+        // ---- weights: p' = exp2(s + log2(vs) - m) ----
+        // m is a reference that need not be the maximum, only near it: it moves when a value
+        // passes 2^kMost, where f16 would end, so most tiles neither reduce over lanes nor touch O.
+        const bool masked = t0 + kTile - 1 > first_last;
+        uint2 P[N][2];      // B fragments of the two 16-key steps
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+          const float f[2][2] = {{ks.x * qs[t][0], ks.x * qs[t][1]}, {ks.y * qs[t][0], ks.y * qs[t][1]}};
+          // Value e of S[t][mt]: key 16 mt + 8 (e / 2) + key_of(g), row 8 t + 2 c + e % 2.
+          if (kSums) {
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e) {
+                const int row = 8 * t + 2 * c + (e & 1), key = t0 + 16 * mt + 8 * (e >> 1) + kg;
+                if (row < rows && key < s.len) {
                   const int q = row_base + row, qi = q / p.G;
-                  p.logits[((int64_t)(s.r0 + qi) * p.Hq + h * p.G + q - qi * p.G) * p.max_ctx + t] = x;
+                  p.logits[((int64_t)(s.r0 + qi) * p.Hq + h * p.G + q - qi * p.G) * p.max_ctx + key] =
+                      key > last[t][e & 1] ? -INFINITY : S[t][mt][e] * f[mt][e & 1];
                 }
               }
-              x += lv[nt >> 1];
-              S[r][nt][e] = x;
-              mx[e >> 1] = fmaxf(mx[e >> 1], x);
+          }
+          float x[2][4];
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              x[mt][e] = fmaf(S[t][mt][e], f[mt][e & 1], (mt == 0 ? lv.x : lv.y) - m[t][e & 1]);
+          if (masked) {
+            __syncwarp();       // keeps this a branch: as selects it would cost every tile
+#pragma unroll
+            for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (t0 + 16 * mt + 8 * (e >> 1) + kg > last[t][e & 1]) x[mt][e] = -INFINITY;
+          }
+          const float mx = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
+                                 fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
+          if (__any_sync(0xffffffffu, mx > kMost)) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              // The row's largest value of this tile, without the old reference.
+              float top = -INFINITY;
+#pragma unroll
+              for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                for (int i2 = e; i2 < 4; i2 += 2)
+                  if (x[mt][i2] != -INFINITY)
+                    top = fmaxf(top, fmaf(S[t][mt][i2], f[mt][e], mt == 0 ? lv.x : lv.y));
+#pragma unroll
+              for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+              const float now = fmaxf(m[t][e], top - kShift);
+              if (now > m[t][e]) {
+                const float alpha = ex2(m[t][e] - now);
+                l[t][e] *= alpha;
+#pragma unroll
+                for (int d = 0; d < 8; ++d) {
+                  O[t][d][e] *= alpha;
+                  O[t][d][2 + e] *= alpha;
+                }
+                m[t][e] = now;
+#pragma unroll
+                for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+                  for (int i2 = e; i2 < 4; i2 += 2)
+                    if (x[mt][i2] != -INFINITY)
+                      x[mt][i2] = fmaf(S[t][mt][i2], f[mt][e], (mt == 0 ? lv.x : lv.y) - now);
+              }
             }
-          bool grew = false;
-          float alpha[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 1));
-            mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], 2));
-            const float now = fmaxf(m[r][e], mx[e]);
-            grew |= now > m[r][e];
-            alpha[e] = now == -INFINITY ? 1.f : ex2(m[r][e] - now);
-            m[r][e] = now;
           }
-          if (__any_sync(0xffffffffu, grew)) {
 #pragma unroll
-            for (int t = 0; t < 16; ++t)
+          for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
-              for (int e = 0; e < 4; ++e) O[r][t][e] *= alpha[e >> 1];
-            l[r][0] *= alpha[0];
-            l[r][1] *= alpha[1];
+            for (int e = 0; e < 4; ++e) x[mt][e] = ex2(x[mt][e]);
+            const float inv = fabsf(mt == 0 ? iv.x : iv.y);
+            l[t][0] = fmaf(x[mt][0] + x[mt][2], inv, l[t][0]);
+            l[t][1] = fmaf(x[mt][1] + x[mt][3], inv, l[t][1]);
+            const __half2 p0 = __floats2half2_rn(x[mt][0], x[mt][1]), p1 = __floats2half2_rn(x[mt][2], x[mt][3]);
+            P[t][mt] = make_uint2(transpose8(*reinterpret_cast<const uint32_t*>(&p0)),
+                                  transpose8(*reinterpret_cast<const uint32_t*>(&p1)));
           }
-          float off[2], add[2][2] = {};
-#pragma unroll
-          for (int e = 0; e < 2; ++e) off[e] = m[r][e] == -INFINITY ? 0.f : m[r][e] - kShift;
-          uint32_t pw[4][2];
-#pragma unroll
-          for (int nt = 0; nt < 4; ++nt) {
-            float x[4];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              x[e] = ex2(S[r][nt][e] - off[e >> 1]);
-              add[nt >> 1][e >> 1] += x[e];
-            }
-            const __half2 p0 = __floats2half2_rn(x[0], x[1]), p1 = __floats2half2_rn(x[2], x[3]);
-            pw[nt][0] = *reinterpret_cast<const uint32_t*>(&p0);
-            pw[nt][1] = *reinterpret_cast<const uint32_t*>(&p1);
-          }
-          const float iv[2] = {__fdividef(1.f, sc.z), __fdividef(1.f, sc.w)};
-#pragma unroll
-          for (int e = 0; e < 2; ++e) l[r][e] += add[0][e] * iv[0] + add[1][e] * iv[1];
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-            P[r][j] = make_uint4(pw[2 * j][0], pw[2 * j][1], pw[2 * j + 1][0], pw[2 * j + 1][1]);
         }
-        // ---- O += P V ----
+        // ---- O^T += V^T P^T: tile d of O is values 16 g + 2 d and one more of the head ----
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           uint4 v[4];
@@ -455,88 +518,105 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
           for (int e = 0; e < 4; ++e) {
             const int key = 8 * (2 * j + (e >> 1)) + key_of(2 * c + (e & 1));
             v[e] = *reinterpret_cast<const uint4*>(vt + key * kv8::kD + ((g ^ (key & 7)) << 4));
-            if (tail && t0 + key >= v_end[j]) v[e] = make_uint4(0, 0, 0, 0);
           }
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const uint32_t w[4] = {q == 0 ? v[0].x : q == 1 ? v[0].y : q == 2 ? v[0].z : v[0].w,
-                                   q == 0 ? v[1].x : q == 1 ? v[1].y : q == 2 ? v[1].z : v[1].w,
-                                   q == 0 ? v[2].x : q == 1 ? v[2].y : q == 2 ? v[2].z : v[2].w,
-                                   q == 0 ? v[3].x : q == 1 ? v[3].y : q == 2 ? v[3].z : v[3].w};
+          for (int q = 0; q < 4; ++q)
 #pragma unroll
             for (int half = 0; half < 2; ++half) {    // values 2 half and 2 half + 1 of the four
-              // Bytes of the two keys side by side as `convert` pairs them.
+              // Bytes of two keys side by side as `convert` pairs them.
               constexpr uint32_t kSel[2][2] = {{0x5410, 0x7632}, {0x5140, 0x7362}};
-              const uint32_t x = __byte_perm(w[0], w[1], kSel[kKind][half]);
-              const uint32_t y = __byte_perm(w[2], w[3], kSel[kKind][half]);
-              uint32_t x0, x1, y0, y1;
-              convert<kKind>(x, x0, x1);
-              convert<kKind>(y, y0, y1);
+              const uint32_t x = __byte_perm(word_of(v[0], q), word_of(v[1], q), kSel[kKind][half]);
+              const uint32_t y = __byte_perm(word_of(v[2], q), word_of(v[3], q), kSel[kKind][half]);
+              uint32_t a0, a1, a2, a3;
+              convert<kKind>(x, a0, a1);
+              convert<kKind>(y, a2, a3);
 #pragma unroll
-              for (int r = 0; r < R; ++r) {
-                mma_f16(O[r][4 * q + 2 * half], P[r][j], x0, y0);
-                mma_f16(O[r][4 * q + 2 * half + 1], P[r][j], x1, y1);
-              }
+              for (int t = 0; t < N; ++t) mma_f16(O[t][2 * q + half], a0, a1, a2, a3, P[t][j].x, P[t][j].y);
             }
-          }
         }
       }
       __syncwarp();               // the stage has been read by every lane
       issue(i + kStages);
     }
 
-    // ---- join the four warps ----
+    // ---- join the four warps: 2 and 3 hand theirs to 0 and 1, then 1 to 0 ----
 #pragma unroll
-    for (int r = 0; r < R; ++r)
+    for (int t = 0; t < N; ++t)
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        l[r][e] += __shfl_xor_sync(0xffffffffu, l[r][e], 1);
-        l[r][e] += __shfl_xor_sync(0xffffffffu, l[r][e], 2);
-        const int row = 16 * r + 8 * e + g;
-        if (c == 0) {
-          sh.m[warp][row] = m[r][e];
-          sh.l[warp][row] = l[r][e];
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], o);
+#pragma unroll
+    for (int from = 2; from > 0; --from) {        // warps [from, 2 from) give, [0, from) take
+      __syncthreads();
+      if (warp >= from && warp < 2 * from) {
+#pragma unroll
+        for (int t = 0; t < N; ++t) {
+#pragma unroll
+          for (int d = 0; d < 8; ++d)
+            sh.o[warp - from][t][d][lane] = make_float4(O[t][d][0], O[t][d][1], O[t][d][2], O[t][d][3]);
+          if (g == 0) {
+            sh.ml[warp - from][8 * t + 2 * c] = make_float2(m[t][0], l[t][0]);
+            sh.ml[warp - from][8 * t + 2 * c + 1] = make_float2(m[t][1], l[t][1]);
+          }
         }
-        // Lane (g, c) holds values 32 c .. 32 c + 31 of its rows.
-        float4* dst = reinterpret_cast<float4*>(&sh.o[warp][row][36 * c]);
+      }
+      __syncthreads();
+      if (warp < from) {
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-          dst[q] = make_float4(O[r][4 * q][2 * e], O[r][4 * q + 1][2 * e], O[r][4 * q + 2][2 * e], O[r][4 * q + 3][2 * e]);
-          dst[4 + q] = make_float4(O[r][4 * q][2 * e + 1], O[r][4 * q + 1][2 * e + 1], O[r][4 * q + 2][2 * e + 1],
-                                   O[r][4 * q + 3][2 * e + 1]);
+        for (int t = 0; t < N; ++t) {
+          float mine[2], theirs[2];
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const float2 ml = sh.ml[warp][8 * t + 2 * c + e];
+            const float now = fmaxf(m[t][e], ml.x);
+            mine[e] = m[t][e] == -INFINITY ? 0.f : ex2(m[t][e] - now);
+            theirs[e] = ml.x == -INFINITY ? 0.f : ex2(ml.x - now);
+            m[t][e] = now;
+            l[t][e] = l[t][e] * mine[e] + ml.y * theirs[e];
+          }
+#pragma unroll
+          for (int d = 0; d < 8; ++d) {
+            const float4 x = sh.o[warp][t][d][lane];
+            O[t][d][0] = O[t][d][0] * mine[0] + x.x * theirs[0];
+            O[t][d][1] = O[t][d][1] * mine[1] + x.y * theirs[1];
+            O[t][d][2] = O[t][d][2] * mine[0] + x.z * theirs[0];
+            O[t][d][3] = O[t][d][3] * mine[1] + x.w * theirs[1];
+          }
         }
       }
-    __syncthreads();
-    const bool whole = unit0 == 0 && stop == item0 + units;
-    const int slot = 2 * blockIdx.x + (item0 + unit0 == first ? 0 : 1);
-    for (int e = tid; e < rows * 32; e += kThreads) {
-      const int row = e >> 5, d4 = e & 31;          // four values a thread
-      float mx = -INFINITY;
+    }
+    if (warp == 0) {
+      const bool whole = unit0 == 0 && stop == item0 + units;
+      const int slot = 2 * blockIdx.x + (item0 + unit0 == first ? 0 : 1);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) mx = fmaxf(mx, sh.m[w][row]);
-      float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-      float sum = 0.f;
+      for (int t = 0; t < N; ++t)
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float f = mx == -INFINITY ? 0.f : ex2(sh.m[w][row] - mx);
-        const float4 x = *reinterpret_cast<const float4*>(&sh.o[w][row][4 * d4 + 4 * (d4 >> 3)]);
-        o.x += f * x.x;
-        o.y += f * x.y;
-        o.z += f * x.z;
-        o.w += f * x.w;
-        sum += f * sh.l[w][row];
-      }
-      if (whole) {
-        const int q = row_base + row, qi = q / p.G;
-        const int64_t at = (int64_t)(s.r0 + qi) * p.Hq + h * p.G + q - qi * p.G;
-        const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;      // NaN stays NaN
-        *reinterpret_cast<uint2*>(p.out + at * kv8::kD + 4 * d4) =
-            make_uint2(mes::pack_bf16x2(o.x * inv, o.y * inv), mes::pack_bf16x2(o.z * inv, o.w * inv));
-        if (kSums && d4 == 0) p.lse[at] = mx - kShift + log2f(sum);
-      } else {
-        *reinterpret_cast<float4*>(p.part_o + ((int64_t)slot * kRows + row) * kv8::kD + 4 * d4) = o;
-        if (d4 == 0) p.part_ml[(int64_t)slot * kRows + row] = make_float2(mx, sum);
-      }
+        for (int e = 0; e < 2; ++e) {
+          const int row = 8 * t + 2 * c + e;
+          if (row >= rows) continue;
+          if (whole) {
+            const int q = row_base + row, qi = q / p.G;
+            const int64_t at = (int64_t)(s.r0 + qi) * p.Hq + h * p.G + q - qi * p.G;
+            const float inv = l[t][e] > 0.f ? 1.f / l[t][e] : l[t][e] == 0.f ? 0.f : l[t][e];      // NaN stays NaN
+            uint4* dst = reinterpret_cast<uint4*>(p.out + at * kv8::kD + 16 * g);
+#pragma unroll
+            for (int q4 = 0; q4 < 2; ++q4) {
+              uint32_t w[4];
+#pragma unroll
+              for (int d = 0; d < 4; ++d)
+                w[d] = mes::pack_bf16x2(O[t][4 * q4 + d][e] * inv, O[t][4 * q4 + d][2 + e] * inv);
+              dst[q4] = make_uint4(w[0], w[1], w[2], w[3]);
+            }
+            if (kSums && g == 0) p.lse[at] = m[t][e] + log2f(l[t][e]);
+          } else {
+            float4* dst = reinterpret_cast<float4*>(p.part_o + ((int64_t)slot * kRows + row) * kv8::kD + 16 * g);
+#pragma unroll
+            for (int q4 = 0; q4 < 4; ++q4)
+              dst[q4] = make_float4(O[t][2 * q4][e], O[t][2 * q4][2 + e], O[t][2 * q4 + 1][e], O[t][2 * q4 + 1][2 + e]);
+            if (g == 0) p.part_ml[(int64_t)slot * kRows + row] = make_float2(m[t][e], l[t][e]);
+          }
+        }
     }
   }
   if (!ok) {
@@ -548,58 +628,120 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
   }
 }
 
-// ---- join the partial results of items cut between blocks: a warp for each (token, query head) ----
-template <int R, bool kSums>
-__global__ void __launch_bounds__(128)
+// ---- join the partial results of items cut between blocks: W warps for each (token, query head) ----
+template <int N, int W, bool kSums>
+__global__ void __launch_bounds__(kThreads)
 kv8_join_kernel(const Params p, int grid) {
-  constexpr int kRows = 16 * R;
-  const int lane = threadIdx.x & 31;
-  const int64_t at = blockIdx.x * 4ll + (threadIdx.x >> 5);
+  constexpr int kRows = 8 * N;
+  __shared__ float4 part[kWarps][32];
+  __shared__ float2 part_ml[kWarps];
+  if (kSums) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t at = blockIdx.x * (int64_t)(kWarps / W) + warp / W;
   if (at >= (int64_t)p.T * p.Hq) return;
   const int token = (int)(at / p.Hq), head = (int)(at - (int64_t)token * p.Hq), h = head / p.G;
-  int lo = 0, hi = p.B;                       // cu[lo] <= token < cu[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) >> 1;
-    if (p.cu[mid] <= token) lo = mid; else hi = mid;
+  // The token's sequence and the units before it and in all, from the lengths alone: this part
+  // runs while the attention kernel does.
+  Seq s = {0, 0, 0};
+  int total = 0, before = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    Seq x = {0, 0, 0};
+    if (b0 + lane < p.B) x = sequence(p, b0 + lane);
+    const int mine = x.n > 0 ? units_of(x.len) * p.Hkv * row_tiles<N>(x.n, p.G) : 0;
+    total += __reduce_add_sync(0xffffffffu, mine);
+    before += __reduce_add_sync(0xffffffffu, x.r0 + x.n <= token ? mine : 0);
+    const uint32_t found = __ballot_sync(0xffffffffu, x.n > 0 && token >= x.r0 && token < x.r0 + x.n);
+    if (found) {
+      const int src = __ffs(found) - 1;
+      s.r0 = __shfl_sync(0xffffffffu, x.r0, src);
+      s.n = __shfl_sync(0xffffffffu, x.n, src);
+      s.len = __shfl_sync(0xffffffffu, x.len, src);
+    }
   }
-  const Seq s = sequence(p, lo);
-  if (s.n <= 0 || token < s.r0 || token >= s.r0 + s.n) return;
-  const int total = p.prefix_out[p.B], blocks = min(grid, total);
+  if (s.n <= 0) return;
+  const int blocks = min(grid, total);
   const int row = (token - s.r0) * p.G + head - h * p.G, tile = row / kRows;
   const int units = units_of(s.len);
-  const int u0 = p.prefix_out[lo] + (h * row_tiles<R>(s.n, p.G) + tile) * units, u1 = u0 + units;
+  const int u0 = before + (h * row_tiles<N>(s.n, p.G) + tile) * units, u1 = u0 + units;
   // The blocks whose shares meet [u0, u1).
   int from = (int)((int64_t)u0 * blocks / total);
   while (from + 1 < blocks && share(total, from + 1, blocks) <= u0) ++from;
   while (from > 0 && share(total, from, blocks) > u0) --from;
   if (share(total, from + 1, blocks) >= u1) return;         // not cut
+  const int to = [&] {                                     // one past the last of them
+    int i = (int)((int64_t)(u1 - 1) * blocks / total);
+    while (i + 1 < blocks && share(total, i + 1, blocks) < u1) ++i;
+    while (share(total, i, blocks) >= u1) --i;
+    return i + 1;
+  }();
+  const int local = row - tile * kRows;
+  // Only the item's first block can have it as its second segment.
+  auto slot = [&](int i) { return ((int64_t)2 * i + (i == from && share(total, i, blocks) < u0 ? 1 : 0)) * kRows + local; };
+  asm volatile("griddepcontrol.wait;" ::: "memory");       // the partial results are there
+  // Each of the W warps takes every W-th partial result; its loads do not wait for one another.
   float mx = -INFINITY, sum = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i = from; i < blocks; ++i) {
-    const int begin = share(total, i, blocks);
-    if (begin >= u1) break;
-    const int64_t slot = ((int64_t)2 * i + (begin < u0 ? 1 : 0)) * kRows + row - tile * kRows;
-    const float2 ml = p.part_ml[slot];
-    const float4 x = *reinterpret_cast<const float4*>(p.part_o + slot * kv8::kD + 4 * lane);
-    const float now = fmaxf(mx, ml.x);
-    if (now == -INFINITY) continue;
-    const float a = ex2(mx - now), f = ex2(ml.x - now);
-    o.x = o.x * a + x.x * f;
-    o.y = o.y * a + x.y * f;
-    o.z = o.z * a + x.z * f;
-    o.w = o.w * a + x.w * f;
-    sum = sum * a + ml.y * f;
+  for (int i0 = from + warp % W; i0 < to; i0 += 8 * W) {
+    float2 ml[8];
+    float4 x[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      ml[j] = make_float2(-INFINITY, 0.f);
+      x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (i0 + j * W < to) {
+        ml[j] = p.part_ml[slot(i0 + j * W)];
+        x[j] = *reinterpret_cast<const float4*>(p.part_o + slot(i0 + j * W) * kv8::kD + 4 * lane);
+      }
+    }
+    float now = mx;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) now = fmaxf(now, ml[j].x);
+    const float keep = mx == -INFINITY ? 0.f : ex2(mx - now);
+    sum *= keep;
+    o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const float f = ml[j].x == -INFINITY ? 0.f : ex2(ml[j].x - now);
+      sum += f * ml[j].y;
+      o.x += f * x[j].x;
+      o.y += f * x[j].y;
+      o.z += f * x[j].z;
+      o.w += f * x[j].w;
+    }
     mx = now;
+  }
+  if (W > 1) {
+    part[warp][lane] = o;
+    if (lane == 0) part_ml[warp] = make_float2(mx, sum);
+    __syncthreads();                // W == kWarps: the block's warps have all come here
+    if (warp != 0) return;
+    mx = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < W; ++w) mx = fmaxf(mx, part_ml[w].x);
+    sum = 0.f;
+    o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < W; ++w) {
+      const float2 ml = part_ml[w];
+      const float4 x = part[w][lane];
+      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - mx);
+      sum += f * ml.y;
+      o.x += f * x.x;
+      o.y += f * x.y;
+      o.z += f * x.z;
+      o.w += f * x.w;
+    }
   }
   const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
   *reinterpret_cast<uint2*>(p.out + at * kv8::kD + 4 * lane) =
       make_uint2(mes::pack_bf16x2(o.x * inv, o.y * inv), mes::pack_bf16x2(o.z * inv, o.w * inv));
-  if (kSums && lane == 0) p.lse[at] = mx - kShift + log2f(sum);
+  if (kSums && lane == 0) p.lse[at] = mx + log2f(sum);
 }
 
 // ---- sums[t] += sum over the rows of a kv head of exp2(logit - lse): a thread for each key ----
 __global__ void __launch_bounds__(256)
 kv8_sums_kernel(const Params p, float* sums) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t b = blockIdx.y / p.Hkv;
   const int h = (int)(blockIdx.y - b * p.Hkv);
   const Seq s = sequence(p, (int)b);
@@ -619,20 +761,19 @@ kv8_sums_kernel(const Params p, float* sums) {
   *at += add;
 }
 
-// Row tiles of 32 are for calls whose kv heads have more than 16 query rows: the converted keys
-// then feed twice the products.
-int row_tile_factor(int64_t max_new, int G) { return max_new * G > 16 ? 2 : 1; }
-int max_blocks(int R) { return mes_host::sm_count() * blocks_per_sm(R); }
+// Row tiles as large as the most query rows of a kv head, at most 32: a converted key feeds one
+// product for each 8 rows.
+int row_factor(int64_t max_new, int G) { return max_new * G <= 8 ? 1 : max_new * G <= 16 ? 2 : 4; }
+int max_blocks(int N) { return mes_host::sm_count() * blocks_per_sm(N); }
 
 constexpr int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
 struct Layout {
-  int64_t prefix, part_o, part_ml, lse, logits, bytes;
+  int64_t part_o, part_ml, lse, logits, bytes;
 };
-Layout layout(int64_t T, int64_t B, int Hq, int R, int64_t max_ctx) {
+Layout layout(int64_t T, int Hq, int N, int64_t max_ctx) {
   Layout w;
-  const int64_t slots = 2ll * max_blocks(R) * 16 * R;
-  w.prefix = 0;
-  w.part_o = up256(4 * (B + 1));
+  const int64_t slots = 2ll * max_blocks(N) * 8 * N;
+  w.part_o = 0;
   w.part_ml = w.part_o + slots * kv8::kD * 4;
   w.lse = up256(w.part_ml + slots * 8);
   w.logits = up256(w.lse + (max_ctx > 0 ? 4 * T * Hq : 0));
@@ -644,23 +785,41 @@ bool valid_sizes(int64_t T, int64_t B, int Hq, int Hkv, int64_t max_new, int64_t
          max_new >= 0 && max_new <= T && T <= 0x7fffffffll / Hq && max_ctx >= 0 && max_ctx <= 0x7fffffffll;
 }
 
-template <int kKind, int R, bool kSums>
+template <int kKind, int N, bool kSums>
 int launch(const CUtensorMap& map, const Params& p, float* sums, void* stream) {
-  auto kernel = kv8_attention_kernel<kKind, R, kSums>;
-  const size_t smem = sizeof(Smem<R>) + 1024;
+  auto kernel = kv8_attention_kernel<kKind, N, kSums>;
   static std::atomic<uint64_t> configured{0};
   int st = mes_host::once_per_device(configured, [&] {
     return mes_host::from_cuda(
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<N>(kMaxSeqs)));
   });
   if (st != MES_OK) return st;
-  const int grid = mes_host::persistent_ctas() * blocks_per_sm(R);
-  kernel<<<grid, kThreads, smem, (cudaStream_t)stream>>>(map, p);
-  const int64_t rows = (int64_t)p.T * p.Hq;
-  kv8_join_kernel<R, kSums><<<(unsigned)((rows + 3) / 4), 128, 0, (cudaStream_t)stream>>>(p, grid);
-  if (kSums)
-    kv8_sums_kernel<<<dim3((unsigned)((p.max_ctx + 255) / 256), (unsigned)(p.B * p.Hkv)), 256, 0, (cudaStream_t)stream>>>(p, sums);
-  return mes_host::from_cuda(cudaGetLastError());
+  // As many blocks an SM as fit (many sequences take one's place); 1 KB of each is the system's.
+  const int fit = (int)(233472 / (smem_bytes<N>(p.B) + 1024));
+  const int grid = mes_host::persistent_ctas() * (fit < blocks_per_sm(N) ? fit : blocks_per_sm(N));
+  kernel<<<grid, kThreads, smem_bytes<N>(p.B), (cudaStream_t)stream>>>(map, p);
+  if (cudaGetLastError() != cudaSuccess) return MES_ERR_CUDA;
+  // The kernels that follow start while the one before them ends (programmatic launch).
+  cudaLaunchAttribute attr = {};
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.stream = (cudaStream_t)stream;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  // Few items leave many partial results each: four warps then share a row's.
+  const bool wide = (int64_t)p.B * p.Hkv * 4 <= grid;
+  const int per_block = wide ? 1 : kWarps;
+  cfg.gridDim = dim3((unsigned)(((int64_t)p.T * p.Hq + per_block - 1) / per_block));
+  cfg.blockDim = dim3(kThreads);
+  if (cudaLaunchKernelEx(&cfg, wide ? kv8_join_kernel<N, kWarps, kSums> : kv8_join_kernel<N, 1, kSums>, p, grid) != cudaSuccess)
+    return MES_ERR_CUDA;
+  if (kSums) {
+    cfg.gridDim = dim3((unsigned)((p.max_ctx + 255) / 256), (unsigned)(p.B * p.Hkv));
+    cfg.blockDim = dim3(256);
+    if (cudaLaunchKernelEx(&cfg, kv8_sums_kernel, p, sums) != cudaSuccess) return MES_ERR_CUDA;
+  }
+  return MES_OK;
 }
 
 }  // namespace
@@ -677,7 +836,7 @@ extern "C" int mes_kv8_attention_take_error(int* code) {
 extern "C" int64_t mes_kv8_attention_workspace_size(int64_t T, int64_t B, int Hq, int Hkv, int64_t max_new,
                                                     int64_t max_context) {
   if (!valid_sizes(T, B, Hq, Hkv, max_new, max_context)) return -1;
-  return layout(T, B, Hq, row_tile_factor(max_new, Hq / Hkv), max_context).bytes;
+  return layout(T, Hq, row_factor(max_new, Hq / Hkv), max_context).bytes;
 }
 
 extern "C" int mes_kv8_attention(int dtype, const void* q, int64_t ldq, const void* codes, const float* scales,
@@ -696,11 +855,11 @@ extern "C" int mes_kv8_attention(int dtype, const void* q, int64_t ldq, const vo
       !kv8::aligned(block_table, 4) || !kv8::aligned(cu_new, 4) || !kv8::aligned(context_lens, 4) ||
       !kv8::aligned(out, 16) || !kv8::aligned(workspace, 256))
     return MES_ERR_ALIGN;
-  const int G = Hq / Hkv, R = row_tile_factor(max_new, G);
-  const Layout w = layout(T, B, Hq, R, max_ctx);
+  const int G = Hq / Hkv, N = row_factor(max_new, G);
+  const Layout w = layout(T, Hq, N, max_ctx);
   if (workspace_bytes < w.bytes) return MES_ERR_INVALID;
   // Units are counted in 32 bits.
-  const int64_t tiles = (max_new * G + 16 * R - 1) / (16 * R);
+  const int64_t tiles = (max_new * G + 8 * N - 1) / (8 * N);
   if (((table_width * page_size + kUnit - 1) / kUnit) * Hkv > 0x7fffffffll / (B * tiles)) return MES_ERR_INVALID;
   if (sums && B * Hkv > 65535) return MES_ERR_INVALID;
   CUtensorMap map;
@@ -727,17 +886,17 @@ extern "C" int mes_kv8_attention(int dtype, const void* q, int64_t ldq, const vo
   p.num_pages = num_pages;
   p.scale = scale;
   p.out = (__nv_bfloat16*)out;
-  p.prefix_out = (int*)(ws + w.prefix);
   p.part_o = (float*)(ws + w.part_o);
   p.part_ml = (float2*)(ws + w.part_ml);
   p.lse = sums ? (float*)(ws + w.lse) : nullptr;
   p.logits = sums ? (float*)(ws + w.logits) : nullptr;
   p.max_ctx = max_ctx;
-  const bool i8 = dtype == kv8::kInt8;
-  if (R == 1) {
-    if (sums) return i8 ? launch<kv8::kInt8, 1, true>(map, p, sums, stream) : launch<kv8::kE4m3, 1, true>(map, p, sums, stream);
-    return i8 ? launch<kv8::kInt8, 1, false>(map, p, sums, stream) : launch<kv8::kE4m3, 1, false>(map, p, sums, stream);
-  }
-  if (sums) return i8 ? launch<kv8::kInt8, 2, true>(map, p, sums, stream) : launch<kv8::kE4m3, 2, true>(map, p, sums, stream);
-  return i8 ? launch<kv8::kInt8, 2, false>(map, p, sums, stream) : launch<kv8::kE4m3, 2, false>(map, p, sums, stream);
+  auto go = [&](auto n) {
+    constexpr int kN = decltype(n)::value;
+    if (dtype == kv8::kInt8)
+      return sums ? launch<kv8::kInt8, kN, true>(map, p, sums, stream) : launch<kv8::kInt8, kN, false>(map, p, sums, stream);
+    return sums ? launch<kv8::kE4m3, kN, true>(map, p, sums, stream) : launch<kv8::kE4m3, kN, false>(map, p, sums, stream);
+  };
+  return N == 1 ? go(std::integral_constant<int, 1>()) : N == 2 ? go(std::integral_constant<int, 2>())
+                                                               : go(std::integral_constant<int, 4>());
 }
