@@ -10,6 +10,7 @@ CUDA device is present, the call raises.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 
 import torch
@@ -513,26 +514,44 @@ def awq_gemm(x: torch.Tensor, qweight_mes: torch.Tensor, qzeros: torch.Tensor,
 
 # --------------------------------------------------------------------------------------
 # Token steps: matrix-vector products and the 8-bit paged KV cache
+#
+# A token step's kernels take a few microseconds each, so what these wrappers do on the host
+# counts: the checks below are one expression each over the attributes that a valid call has,
+# and only when it is false do the checks of the wrappers above run, which name what is wrong
+# (and pass CPU tensors on to ``_stream``).
 # --------------------------------------------------------------------------------------
 GEMV_MAX_ROWS = 16
+_BF16, _F32, _I32T = torch.bfloat16, torch.float32, torch.int32
 
 
-def _awq_gemv_call(epi: int, x: torch.Tensor, qweight_mes: torch.Tensor, qzeros: torch.Tensor,
-                   scales: torch.Tensor, bias, y: torch.Tensor, group_size: int) -> None:
-    _awq_args(qweight_mes, qzeros, scales, x, group_size)
-    K, N = qweight_mes.shape[0] * 8, qweight_mes.shape[1]
-    _arg(bias, "bias", x, torch.bfloat16, (N,), contiguous=True)
-    _check(lib().mes_awq_gemv(epi, _p(x), x.stride(0), _p(qweight_mes), _p(qzeros), _p(scales),
-                              _p(bias), _p(y), y.stride(0), x.shape[0], N, K, group_size,
-                              _stream(x)), f"mes_awq_gemv ({_EPI_NAME[epi]} epilogue)")
+def _gemv_args(x: torch.Tensor, qw: torch.Tensor, qz: torch.Tensor, sc: torch.Tensor,
+               group_size: int):
+    """Checks the operands of a matrix-vector product; returns its ``(M, N, K)``."""
+    dev = x.get_device()
+    M, K = x.shape if x.dim() == 2 else (-1, -1)
+    N = qw.shape[-1]
+    if not (dev >= 0 and dev == qw.get_device() and dev == qz.get_device() and dev == sc.get_device()
+            and x.dtype is _BF16 and qw.dtype is _I32T and qz.dtype is _I32T and sc.dtype in _SCALES
+            and 0 <= M <= GEMV_MAX_ROWS and group_size > 0 and qw.shape == (K // 8, N) and K % 8 == 0
+            and qz.shape == (K // group_size, N // 8) and sc.shape == (K // group_size, N)
+            and qw.is_contiguous() and qz.is_contiguous() and sc.is_contiguous() and x.stride()[1] == 1):
+        _need(x.dtype == torch.bfloat16 and x.dim() == 2 and x.stride(-1) == 1,
+              "x must be bf16 [M, K] with unit inner stride")
+        _need(M <= GEMV_MAX_ROWS, f"x has {M} rows, at most {GEMV_MAX_ROWS} are taken")
+        _need(qw.dim() == 2 and K == qw.shape[0] * 8, f"x has K={K}, the weight is {tuple(qw.shape)}")
+        _awq_args(qw, qz, sc, x, group_size)
+        _arg(qw, "qweight_mes", x)
+    return M, N, K
 
 
-def _gemv_x(x: torch.Tensor, qweight_mes: torch.Tensor) -> None:
-    _need(x.dtype == torch.bfloat16 and x.dim() == 2 and x.stride(-1) == 1,
-          "x must be bf16 [M, K] with unit inner stride")
-    _need(x.shape[0] <= GEMV_MAX_ROWS, f"x has {x.shape[0]} rows, at most {GEMV_MAX_ROWS} are taken")
-    _need(qweight_mes.dim() == 2 and x.shape[1] == qweight_mes.shape[0] * 8,
-          f"x has K={x.shape[1]}, weight has K={qweight_mes.shape[0] * 8}")
+def _gemv_call(epi: int, x, qw, qz, sc, bias, y, M: int, N: int, K: int, group_size: int) -> None:
+    global launch_count
+    st = lib().mes_awq_gemv(epi, x.data_ptr(), x.stride()[0], qw.data_ptr(), qz.data_ptr(), sc.data_ptr(),
+                            None if bias is None else bias.data_ptr(), y.data_ptr(), y.stride()[0], M, N, K,
+                            group_size, _stream(x))
+    if st:
+        _check(st, f"mes_awq_gemv ({_EPI_NAME[epi]} epilogue)")
+    launch_count += 1
 
 
 def awq_gemv(x: torch.Tensor, qweight_mes: torch.Tensor, qzeros: torch.Tensor,
@@ -540,12 +559,14 @@ def awq_gemv(x: torch.Tensor, qweight_mes: torch.Tensor, qzeros: torch.Tensor,
              out: torch.Tensor | None = None, group_size: int = 128) -> torch.Tensor:
     """``x[M, K] @ W[K, N] (+ bias)`` for at most 16 rows: the projections of a token step
     (``mes_awq_gemv``).  The weights are not rounded to bf16 first, as ``awq_gemm`` does."""
-    _gemv_x(x, qweight_mes)
-    M, N = x.shape[0], qweight_mes.shape[1]
-    _arg(out, "out", x, torch.bfloat16, (M, N), unit_stride=True)
+    M, N, K = _gemv_args(x, qweight_mes, qzeros, scales, group_size)
+    if bias is not None:
+        _arg(bias, "bias", x, torch.bfloat16, (N,), contiguous=True)
     if out is None:
-        out = torch.empty(M, N, dtype=torch.bfloat16, device=x.device)
-    _awq_gemv_call(EPI_BF16, x, qweight_mes, qzeros, scales, bias, out, group_size)
+        out = torch.empty((M, N), dtype=_BF16, device=x.device)
+    else:
+        _arg(out, "out", x, torch.bfloat16, (M, N), unit_stride=True)
+    _gemv_call(EPI_BF16, x, qweight_mes, qzeros, scales, bias, out, M, N, K, group_size)
     return out
 
 
@@ -553,9 +574,13 @@ def awq_gemv_residual(x: torch.Tensor, qweight_mes: torch.Tensor, qzeros: torch.
                       scales: torch.Tensor, residual: torch.Tensor,
                       bias: torch.Tensor | None = None, group_size: int = 128) -> torch.Tensor:
     """``residual[M, N] (fp32) += x @ W (+ bias)`` for at most 16 rows."""
-    _gemv_x(x, qweight_mes)
-    _arg(residual, "residual", x, torch.float32, (x.shape[0], qweight_mes.shape[1]), unit_stride=True)
-    _awq_gemv_call(EPI_RESIDUAL, x, qweight_mes, qzeros, scales, bias, residual, group_size)
+    M, N, K = _gemv_args(x, qweight_mes, qzeros, scales, group_size)
+    if not (residual.dtype is _F32 and residual.shape == (M, N) and residual.get_device() == x.get_device() >= 0
+            and residual.stride()[1] == 1):
+        _arg(residual, "residual", x, torch.float32, (M, N), unit_stride=True)
+    if bias is not None:
+        _arg(bias, "bias", x, torch.bfloat16, (N,), contiguous=True)
+    _gemv_call(EPI_RESIDUAL, x, qweight_mes, qzeros, scales, bias, residual, M, N, K, group_size)
     return residual
 
 
@@ -564,12 +589,12 @@ def awq_gemv_silu(x: torch.Tensor, qweight_mes: torch.Tensor, qzeros: torch.Tens
                   group_size: int = 128) -> torch.Tensor:
     """``silu(x @ Wg) * (x @ Wu)`` for at most 16 rows, gate/up columns interleaved in blocks of
     16 (see ``interleave_gate_up``); output ``[M, N/2]`` bf16."""
-    _gemv_x(x, qweight_mes)
-    M, N = x.shape[0], qweight_mes.shape[1]
-    _arg(out, "out", x, torch.bfloat16, (M, N // 2), unit_stride=True)
+    M, N, K = _gemv_args(x, qweight_mes, qzeros, scales, group_size)
     if out is None:
-        out = torch.empty(M, N // 2, dtype=torch.bfloat16, device=x.device)
-    _awq_gemv_call(EPI_SILU, x, qweight_mes, qzeros, scales, None, out, group_size)
+        out = torch.empty((M, N // 2), dtype=_BF16, device=x.device)
+    else:
+        _arg(out, "out", x, torch.bfloat16, (M, N // 2), unit_stride=True)
+    _gemv_call(EPI_SILU, x, qweight_mes, qzeros, scales, None, out, M, N, K, group_size)
     return out
 
 
@@ -578,25 +603,45 @@ KV8_PAGE_SIZES = (16, 32, 64, 128)
 
 
 def _kv8_cache(codes: torch.Tensor, scales: torch.Tensor, sums: torch.Tensor | None = None):
-    """``(dtype code, num_pages, Hkv, P, D)`` of a cache ``codes [pages, 2, Hkv, P, 128]``,
+    """``(dtype code, num_pages, Hkv, P)`` of a cache ``codes [pages, 2, Hkv, P, 128]``,
     ``scales [pages, 2, Hkv]``, ``sums [pages, Hkv, P]``."""
     kind = KV8_DTYPES.get(codes.dtype)
     _need(kind is not None and codes.dim() == 5, "codes must be int8 or float8_e4m3fn [pages, 2, Hkv, P, 128]")
     pages, two, Hkv, P, D = codes.shape
-    _need(two == 2 and P in KV8_PAGE_SIZES and D == 128 and codes.is_contiguous(),
-          "codes must be contiguous [pages, 2, Hkv, P, 128] with P one of 16, 32, 64, 128")
-    _arg(scales, "scales", codes, torch.float32, (pages, 2, Hkv), contiguous=True)
-    _arg(sums, "sums", codes, torch.float32, (pages, Hkv, P), contiguous=True)
-    return kind, pages, Hkv, P, D
+    dev = codes.get_device()
+    if not (dev >= 0 and two == 2 and D == 128 and P in KV8_PAGE_SIZES and codes.is_contiguous()
+            and scales.dtype is _F32 and scales.shape == (pages, 2, Hkv) and scales.get_device() == dev
+            and scales.is_contiguous() and sums is None):
+        _need(two == 2 and P in KV8_PAGE_SIZES and D == 128 and codes.is_contiguous(),
+              "codes must be contiguous [pages, 2, Hkv, P, 128] with P one of 16, 32, 64, 128")
+        _arg(scales, "scales", codes, torch.float32, (pages, 2, Hkv), contiguous=True)
+        _arg(sums, "sums", codes, torch.float32, (pages, Hkv, P), contiguous=True)
+    return kind, pages, Hkv, P
 
 
-def _kv8_batch(block_table: torch.Tensor, context_lens: torch.Tensor, like: torch.Tensor) -> int:
-    """Checks ``block_table [B, width]`` and ``context_lens [B]`` (int32); returns B."""
+def _kv8_batch(codes: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor,
+               cu_new: torch.Tensor | None = None):
+    """Checks ``block_table [B, width]``, ``context_lens [B]`` and ``cu_new [B + 1]`` (int32);
+    returns ``(B, width)``."""
     _need(block_table.dim() == 2, "block_table must be int32 [B, width]")
-    B = block_table.shape[0]
-    _arg(block_table, "block_table", like, torch.int32, contiguous=True)
-    _arg(context_lens, "context_lens", like, torch.int32, (B,), contiguous=True)
-    return B
+    B, width = block_table.shape
+    dev = codes.get_device()
+    if not (dev >= 0 and block_table.dtype is _I32T and context_lens.dtype is _I32T and block_table.is_contiguous()
+            and block_table.get_device() == dev and context_lens.get_device() == dev
+            and context_lens.shape == (B,) and context_lens.is_contiguous()
+            and (cu_new is None or (cu_new.dtype is _I32T and cu_new.shape == (B + 1,) and cu_new.get_device() == dev
+                                    and cu_new.is_contiguous()))):
+        _arg(block_table, "block_table", codes, torch.int32, contiguous=True)
+        _arg(context_lens, "context_lens", codes, torch.int32, (B,), contiguous=True)
+        _arg(cu_new, "cu_new", codes, torch.int32, (B + 1,), contiguous=True)
+    return B, width
+
+
+def _kv8_rows(t: torch.Tensor, name: str, codes: torch.Tensor, T: int, cols: int) -> None:
+    """Checks the packed rows ``t``: bf16 ``[T, cols]`` of unit inner stride."""
+    if not (t.dtype is _BF16 and t.shape == (T, cols) and t.get_device() == codes.get_device() >= 0
+            and t.stride()[1] == 1):
+        _arg(t, name, codes, torch.bfloat16, (T, cols), unit_stride=True)
 
 
 def kv8_append(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
@@ -606,32 +651,46 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, scales: to
     packed QKV buffer) into the cache (``mes_kv8_append``).  ``cu_new`` int32 ``[B + 1]``:
     offsets of each sequence's rows; ``context_lens`` counts the cached tokens with the new
     ones; ``max_new``: no sequence has more new tokens."""
-    kind, pages, Hkv, P, D = _kv8_cache(codes, scales, sums)
-    B = _kv8_batch(block_table, context_lens, codes)
-    _need(k.dim() == 2, "k must be bf16 [T, Hkv * 128]")
+    global launch_count
+    kind, pages, Hkv, P = _kv8_cache(codes, scales, sums)
+    B, width = _kv8_batch(codes, block_table, context_lens, cu_new)
     T = k.shape[0]
-    _arg(k, "k", codes, torch.bfloat16, (T, Hkv * D), unit_stride=True)
-    _arg(v, "v", codes, torch.bfloat16, (T, Hkv * D), unit_stride=True)
-    _arg(cu_new, "cu_new", codes, torch.int32, (B + 1,), contiguous=True)
-    _check(lib().mes_kv8_append(kind, _p(k), k.stride(0), _p(v), v.stride(0), _p(codes), _p(scales),
-                                _p(sums), _p(block_table), block_table.shape[1], _p(cu_new),
-                                _p(context_lens), B, T, max_new, Hkv, D, P, pages, _stream(codes)),
-           "mes_kv8_append")
+    _kv8_rows(k, "k", codes, T, Hkv * 128)
+    _kv8_rows(v, "v", codes, T, Hkv * 128)
+    st = lib().mes_kv8_append(kind, k.data_ptr(), k.stride()[0], v.data_ptr(), v.stride()[0], codes.data_ptr(),
+                              scales.data_ptr(), None if sums is None else sums.data_ptr(),
+                              block_table.data_ptr(), width, cu_new.data_ptr(), context_lens.data_ptr(), B, T,
+                              max_new, Hkv, 128, P, pages, _stream(codes))
+    if st:
+        _check(st, "mes_kv8_append")
+    launch_count += 1
 
 
 def kv8_read(codes: torch.Tensor, scales: torch.Tensor, pages: torch.Tensor,
              out: torch.Tensor | None = None) -> torch.Tensor:
     """The values of ``pages`` (int32 ``[n]``), bf16 ``[n, 2, Hkv, P, 128]``."""
-    kind, num_pages, Hkv, P, D = _kv8_cache(codes, scales)
+    global launch_count
+    kind, num_pages, Hkv, P = _kv8_cache(codes, scales)
     _need(pages.dim() == 1, "pages must be int32 [n]")
-    _arg(pages, "pages", codes, torch.int32, contiguous=True)
     n = pages.shape[0]
-    _arg(out, "out", codes, torch.bfloat16, (n, 2, Hkv, P, D), contiguous=True)
+    if not (pages.dtype is _I32T and pages.get_device() == codes.get_device() >= 0 and pages.is_contiguous()):
+        _arg(pages, "pages", codes, torch.int32, contiguous=True)
     if out is None:
-        out = torch.empty(n, 2, Hkv, P, D, dtype=torch.bfloat16, device=codes.device)
-    _check(lib().mes_kv8_read(kind, _p(codes), _p(scales), _p(pages), n, Hkv, D, P, num_pages, _p(out),
-                              _stream(codes)), "mes_kv8_read")
+        out = torch.empty((n, 2, Hkv, P, 128), dtype=_BF16, device=codes.device)
+    else:
+        _arg(out, "out", codes, torch.bfloat16, (n, 2, Hkv, P, 128), contiguous=True)
+    st = lib().mes_kv8_read(kind, codes.data_ptr(), scales.data_ptr(), pages.data_ptr(), n, Hkv, 128, P,
+                            num_pages, out.data_ptr(), _stream(codes))
+    if st:
+        _check(st, "mes_kv8_read")
+    launch_count += 1
     return out
+
+
+@functools.lru_cache(maxsize=1024)
+def _kv8_workspace(device: int, *sizes: int) -> int:
+    """``mes_kv8_attention_workspace_size``: the same for the same sizes on one device."""
+    return int(lib().mes_kv8_attention_workspace_size(*sizes))
 
 
 def kv8_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
@@ -641,24 +700,27 @@ def kv8_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     """Causal attention of the new tokens' ``q`` (bf16 rows ``[T, num_heads * 128]``) over the
     cache, their own entries included (``mes_kv8_attention``); bf16 ``[T, num_heads * 128]``.
     With ``sums``, the cached tokens' attention weights are added to it."""
-    kind, pages, Hkv, P, D = _kv8_cache(codes, scales, sums)
-    B = _kv8_batch(block_table, context_lens, codes)
-    _need(q.dim() == 2, "q must be bf16 [T, num_heads * 128]")
-    T, width = q.shape[0], block_table.shape[1]
-    _arg(q, "q", codes, torch.bfloat16, (T, num_heads * D), unit_stride=True)
-    _arg(cu_new, "cu_new", codes, torch.int32, (B + 1,), contiguous=True)
-    _arg(out, "out", codes, torch.bfloat16, (T, num_heads * D), contiguous=True)
+    global launch_count
+    kind, pages, Hkv, P = _kv8_cache(codes, scales, sums)
+    B, width = _kv8_batch(codes, block_table, context_lens, cu_new)
+    T = q.shape[0]
+    _kv8_rows(q, "q", codes, T, num_heads * 128)
     if out is None:
-        out = torch.empty(T, num_heads * D, dtype=torch.bfloat16, device=codes.device)
-    size = int(lib().mes_kv8_attention_workspace_size(T, B, num_heads, Hkv, max_new,
-                                                      0 if sums is None else width * P))
-    _need(size >= 0, f"unsupported sizes: {T} tokens of {B} sequences (at most {max_new} of one), "
-                     f"{num_heads} heads over {Hkv}")
+        out = torch.empty((T, num_heads * 128), dtype=_BF16, device=codes.device)
+    else:
+        _arg(out, "out", codes, torch.bfloat16, (T, num_heads * 128), contiguous=True)
+    size = _kv8_workspace(codes.get_device(), T, B, num_heads, Hkv, max_new, 0 if sums is None else width * P)
+    if size < 0:
+        raise MesError(f"mes_kv8_attention: unsupported sizes: {T} tokens of {B} sequences (at most {max_new} "
+                       f"of one), {num_heads} heads over {Hkv}")
     ws = torch.empty(size, dtype=torch.uint8, device=codes.device)
-    _check(lib().mes_kv8_attention(kind, _p(q), q.stride(0), _p(codes), _p(scales), _p(sums),
-                                   _p(block_table), width, _p(cu_new), _p(context_lens), B, T,
-                                   max_new, num_heads, Hkv, D, P, pages, scale, _p(out), _p(ws), size,
-                                   _stream(codes)), "mes_kv8_attention", 2 if sums is None else 3)
+    st = lib().mes_kv8_attention(kind, q.data_ptr(), q.stride()[0], codes.data_ptr(), scales.data_ptr(),
+                                 None if sums is None else sums.data_ptr(), block_table.data_ptr(), width,
+                                 cu_new.data_ptr(), context_lens.data_ptr(), B, T, max_new, num_heads, Hkv, 128,
+                                 P, pages, scale, out.data_ptr(), ws.data_ptr(), size, _stream(codes))
+    if st:
+        _check(st, "mes_kv8_attention")
+    launch_count += 2 if sums is None else 3
     return out
 
 
@@ -668,15 +730,21 @@ def kv8_evict(codes: torch.Tensor, scales: torch.Tensor, sums: torch.Tensor,
     """Copy each sequence's ``recent`` last tokens and its tokens of largest ``sums`` (per kv
     head), ``keep`` in all, to the pages of ``new_table`` int32 ``[B, ceil(keep / P)]``
     (``mes_kv8_evict``).  Returns ``(kept int32 [B, Hkv, keep], new_lens int32 [B])``."""
-    kind, pages, Hkv, P, D = _kv8_cache(codes, scales, sums)
+    global launch_count
     _need(sums is not None, "sums must be float32 [pages, Hkv, P]")
-    B = _kv8_batch(block_table, context_lens, codes)
+    kind, pages, Hkv, P = _kv8_cache(codes, scales, sums)
+    B, width = _kv8_batch(codes, block_table, context_lens)
     _need(0 <= recent <= keep and keep > 0, "0 <= recent <= keep, keep > 0")
-    _arg(new_table, "new_table", codes, torch.int32, (B, -(-keep // P)), contiguous=True)
-    kept = torch.empty(B, Hkv, keep, dtype=torch.int32, device=codes.device)
-    new_lens = torch.empty(B, dtype=torch.int32, device=codes.device)
-    _check(lib().mes_kv8_evict(kind, _p(codes), _p(scales), _p(sums), _p(block_table),
-                               block_table.shape[1], _p(context_lens), B, _p(new_table),
-                               new_table.shape[1], keep, recent, Hkv, D, P, pages, _p(kept), _p(new_lens),
-                               _stream(codes)), "mes_kv8_evict", 2)
+    new_width = -(-keep // P)
+    if not (new_table.dtype is _I32T and new_table.shape == (B, new_width) and new_table.is_contiguous()
+            and new_table.get_device() == codes.get_device() >= 0):
+        _arg(new_table, "new_table", codes, torch.int32, (B, new_width), contiguous=True)
+    kept = torch.empty((B, Hkv, keep), dtype=_I32T, device=codes.device)
+    new_lens = torch.empty(B, dtype=_I32T, device=codes.device)
+    st = lib().mes_kv8_evict(kind, codes.data_ptr(), scales.data_ptr(), sums.data_ptr(), block_table.data_ptr(),
+                             width, context_lens.data_ptr(), B, new_table.data_ptr(), new_width, keep, recent,
+                             Hkv, 128, P, pages, kept.data_ptr(), new_lens.data_ptr(), _stream(codes))
+    if st:
+        _check(st, "mes_kv8_evict")
+    launch_count += 2
     return kept, new_lens

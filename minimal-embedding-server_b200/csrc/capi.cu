@@ -10,6 +10,7 @@
 extern "C" int mes_elementwise_take_error(int* code);
 extern "C" int mes_gemm_take_error(int* code);
 extern "C" int mes_attention_take_error(int* code);
+extern "C" int mes_awq_gemv_take_error(int* code);
 extern "C" int mes_kv8_cache_take_error(int* code);
 extern "C" int mes_kv8_attention_take_error(int* code);
 
@@ -135,7 +136,7 @@ extern "C" int mes_take_device_error(int* code) {
   *code = 0;
   if (cudaDeviceSynchronize() != cudaSuccess) return MES_ERR_CUDA;
   int (*fns[])(int*) = {mes_elementwise_take_error, mes_gemm_take_error, mes_attention_take_error,
-                        mes_kv8_cache_take_error, mes_kv8_attention_take_error};
+                        mes_awq_gemv_take_error, mes_kv8_cache_take_error, mes_kv8_attention_take_error};
   for (auto f : fns) {
     int c = 0;
     int st = f(&c);

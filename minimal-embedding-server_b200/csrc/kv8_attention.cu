@@ -91,8 +91,7 @@ __device__ __forceinline__ int key_of(int n) {
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                         uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
       "{%8, %9}, {%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -100,7 +99,7 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1,
 // Transposes an 8 x 8 matrix of 16-bit values: lane (g, c) gives row g, columns 2c and 2c + 1.
 __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   uint32_t r;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
@@ -432,12 +431,20 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
         // m is a reference that need not be the maximum, only near it: it moves when a value
         // passes 2^kMost, where f16 would end, so most tiles neither reduce over lanes nor touch O.
         const bool masked = t0 + kTile - 1 > first_last;
-        uint2 P[N][2];      // B fragments of the two 16-key steps
+        // Value e of x[t][mt]: key 16 mt + 8 (e / 2) + key_of(g), row 8 t + 2 c + e % 2.
+        float x[N][2][4], mx = -INFINITY;
 #pragma unroll
-        for (int t = 0; t < N; ++t) {
-          const float f[2][2] = {{ks.x * qs[t][0], ks.x * qs[t][1]}, {ks.y * qs[t][0], ks.y * qs[t][1]}};
-          // Value e of S[t][mt]: key 16 mt + 8 (e / 2) + key_of(g), row 8 t + 2 c + e % 2.
-          if (kSums) {
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              S[t][mt][e] *= (mt == 0 ? ks.x : ks.y) * qs[t][e & 1];
+              x[t][mt][e] = S[t][mt][e] + ((mt == 0 ? lv.x : lv.y) - m[t][e & 1]);
+            }
+        if (kSums) {
+#pragma unroll
+          for (int t = 0; t < N; ++t)
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -446,27 +453,28 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
                 if (row < rows && key < s.len) {
                   const int q = row_base + row, qi = q / p.G;
                   p.logits[((int64_t)(s.r0 + qi) * p.Hq + h * p.G + q - qi * p.G) * p.max_ctx + key] =
-                      key > last[t][e & 1] ? -INFINITY : S[t][mt][e] * f[mt][e & 1];
+                      key > last[t][e & 1] ? -INFINITY : S[t][mt][e];
                 }
               }
-          }
-          float x[2][4];
+        }
+        if (masked) {
+          __syncwarp();       // keeps this a branch: as selects it would cost every tile
 #pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              x[mt][e] = fmaf(S[t][mt][e], f[mt][e & 1], (mt == 0 ? lv.x : lv.y) - m[t][e & 1]);
-          if (masked) {
-            __syncwarp();       // keeps this a branch: as selects it would cost every tile
+          for (int t = 0; t < N; ++t)
 #pragma unroll
             for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
               for (int e = 0; e < 4; ++e)
-                if (t0 + 16 * mt + 8 * (e >> 1) + kg > last[t][e & 1]) x[mt][e] = -INFINITY;
-          }
-          const float mx = fmaxf(fmaxf(fmaxf(x[0][0], x[0][1]), fmaxf(x[0][2], x[0][3])),
-                                 fmaxf(fmaxf(x[1][0], x[1][1]), fmaxf(x[1][2], x[1][3])));
-          if (__any_sync(0xffffffffu, mx > kMost)) {
+                if (t0 + 16 * mt + 8 * (e >> 1) + kg > last[t][e & 1]) x[t][mt][e] = -INFINITY;
+        }
+#pragma unroll
+        for (int t = 0; t < N; ++t)
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+            mx = fmaxf(mx, fmaxf(fmaxf(x[t][mt][0], x[t][mt][1]), fmaxf(x[t][mt][2], x[t][mt][3])));
+        if (__any_sync(0xffffffffu, mx > kMost)) {
+#pragma unroll
+          for (int t = 0; t < N; ++t)
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               // The row's largest value of this tile, without the old reference.
@@ -475,8 +483,7 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
               for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
                 for (int i2 = e; i2 < 4; i2 += 2)
-                  if (x[mt][i2] != -INFINITY)
-                    top = fmaxf(top, fmaf(S[t][mt][i2], f[mt][e], mt == 0 ? lv.x : lv.y));
+                  if (x[t][mt][i2] != -INFINITY) top = fmaxf(top, S[t][mt][i2] + (mt == 0 ? lv.x : lv.y));
 #pragma unroll
               for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
               const float now = fmaxf(m[t][e], top - kShift);
@@ -493,23 +500,24 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
                 for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
                   for (int i2 = e; i2 < 4; i2 += 2)
-                    if (x[mt][i2] != -INFINITY)
-                      x[mt][i2] = fmaf(S[t][mt][i2], f[mt][e], (mt == 0 ? lv.x : lv.y) - now);
+                    if (x[t][mt][i2] != -INFINITY) x[t][mt][i2] = S[t][mt][i2] + ((mt == 0 ? lv.x : lv.y) - now);
               }
             }
-          }
+        }
+        uint2 P[N][2];      // B fragments of the two 16-key steps
+#pragma unroll
+        for (int t = 0; t < N; ++t)
 #pragma unroll
           for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) x[mt][e] = ex2(x[mt][e]);
+            for (int e = 0; e < 4; ++e) x[t][mt][e] = ex2(x[t][mt][e]);
             const float inv = fabsf(mt == 0 ? iv.x : iv.y);
-            l[t][0] = fmaf(x[mt][0] + x[mt][2], inv, l[t][0]);
-            l[t][1] = fmaf(x[mt][1] + x[mt][3], inv, l[t][1]);
-            const __half2 p0 = __floats2half2_rn(x[mt][0], x[mt][1]), p1 = __floats2half2_rn(x[mt][2], x[mt][3]);
+            l[t][0] = fmaf(x[t][mt][0] + x[t][mt][2], inv, l[t][0]);
+            l[t][1] = fmaf(x[t][mt][1] + x[t][mt][3], inv, l[t][1]);
+            const __half2 p0 = __floats2half2_rn(x[t][mt][0], x[t][mt][1]), p1 = __floats2half2_rn(x[t][mt][2], x[t][mt][3]);
             P[t][mt] = make_uint2(transpose8(*reinterpret_cast<const uint32_t*>(&p0)),
                                   transpose8(*reinterpret_cast<const uint32_t*>(&p1)));
           }
-        }
         // ---- O^T += V^T P^T: tile d of O is values 16 g + 2 d and one more of the head ----
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
