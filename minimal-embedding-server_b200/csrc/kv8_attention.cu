@@ -359,6 +359,16 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
         first_last = min(first_last, last[t][e]);
       }
     first_last = __reduce_min_sync(0xffffffffu, first_last);
+    int64_t logit_row[N][2];          // where this lane's rows' logits go, with sums
+    if (kSums) {
+#pragma unroll
+      for (int t = 0; t < N; ++t)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int row = 8 * t + 2 * c + e, q = row_base + row, qi = q / p.G;
+          logit_row[t][e] = row < rows ? ((int64_t)(s.r0 + qi) * p.Hq + h * p.G + q - qi * p.G) * p.max_ctx : -1;
+        }
+    }
     uint2 q1[8];
     if (N == 1) {
 #pragma unroll
@@ -449,12 +459,9 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
             for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
               for (int e = 0; e < 4; ++e) {
-                const int row = 8 * t + 2 * c + (e & 1), key = t0 + 16 * mt + 8 * (e >> 1) + kg;
-                if (row < rows && key < s.len) {
-                  const int q = row_base + row, qi = q / p.G;
-                  p.logits[((int64_t)(s.r0 + qi) * p.Hq + h * p.G + q - qi * p.G) * p.max_ctx + key] =
-                      key > last[t][e & 1] ? -INFINITY : S[t][mt][e];
-                }
+                const int key = t0 + 16 * mt + 8 * (e >> 1) + kg;
+                if (logit_row[t][e & 1] >= 0 && key < s.len)
+                  p.logits[logit_row[t][e & 1] + key] = key > last[t][e & 1] ? -INFINITY : S[t][mt][e];
               }
         }
         if (masked) {

@@ -18,27 +18,71 @@ __device__ __forceinline__ void unpack8(const uint4& v, float (&f)[8]) {
   }
 }
 
+// Eight values -> codes, as `encode(f / scale)` gives them.  The quotients are correctly rounded
+// (Markstein's theorem: with y = RN(1 / b), q within one unit of a / b and r = RN(a - b q), RN(q + r y)
+// is a / b rounded, where nothing underflows; a y may be two units off, a first step brings it
+// within one), which takes five products instead of a division: ties are common among 16-bit
+// values (half of a run's largest value is one), so near is not enough.  `direct`: the scale or
+// the values are outside the range in which that holds.
+struct Divisor {
+  float scale, inv;
+  bool direct;
+};
+__device__ __forceinline__ Divisor divisor(float scale, bool direct) {
+  return {scale, 1.f / scale, direct || !(scale >= 8.6736174e-19f && scale <= 1.2676506e30f)};   // 2^-60, 2^100
+}
+template <int kKind>
+__device__ __forceinline__ uint2 quantise8(const float (&f)[8], const Divisor& by) {
+  uint32_t o[2] = {0, 0};
+  if (by.direct) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) o[e >> 2] |= kv8::encode<kKind>(f[e] / by.scale) << (8 * (e & 3));
+    return make_uint2(o[0], o[1]);
+  }
+  float q[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    q[e] = f[e] * by.inv;
+    q[e] = fmaf(fmaf(-q[e], by.scale, f[e]), by.inv, q[e]);
+    q[e] = fmaf(fmaf(-q[e], by.scale, f[e]), by.inv, q[e]);
+    if (kKind == kv8::kE4m3) q[e] = copysignf(q[e], f[e]);      // the steps turn -0 into 0
+  }
+  // No quotient passes the largest code by more than its rounding.
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    if (kKind == kv8::kInt8) {
+      uint32_t t[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) t[e] = __float_as_uint(q[4 * i + e] + 12582912.f);    // 1.5 2^23: rounds to an integer
+      o[i] = __byte_perm(__byte_perm(t[0], t[1], 0x0040), __byte_perm(t[2], t[3], 0x0040), 0x5410);
+    } else {
+      o[i] = __nv_cvt_float2_to_fp8x2(make_float2(q[4 * i], q[4 * i + 1]), __NV_SATFINITE, __NV_E4M3) |
+             (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(q[4 * i + 2], q[4 * i + 3]), __NV_SATFINITE, __NV_E4M3) << 16;
+    }
+  return make_uint2(o[0], o[1]);
+}
+
 // Rows of one run handled by a warp, and the block shape that follows: a run of P tokens takes
-// P / 16 warps, and a block holds at least four warps, so small pages share a block.
-constexpr int kWarpRows = 16;
-template <int P>
+// P / kRows warps, and a block holds at least four warps, so small pages share a block.
+template <int P, int kRows>
 struct Shape {
-  static constexpr int kRunWarps = P / kWarpRows;
+  static constexpr int kRunWarps = P / kRows;
   static constexpr int kRuns = kRunWarps < 4 ? 4 / kRunWarps : 1;   // runs of a block
   static constexpr int kThreads = 32 * kRunWarps * kRuns;
 };
+constexpr int kAppendRows = 16, kCompactRows = 8;
 
 // Largest value over the warps of a run; every thread of the block calls it.
-template <int P>
+template <int kRunWarps>
 __device__ __forceinline__ float run_max(float v, float* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-  if (Shape<P>::kRunWarps == 1) return v;
-  const int warp = threadIdx.x >> 5, first = warp / Shape<P>::kRunWarps * Shape<P>::kRunWarps;
+  if (kRunWarps == 1) return v;
+  const int warp = threadIdx.x >> 5, first = warp / kRunWarps * kRunWarps;
   if ((threadIdx.x & 31) == 0) red[warp] = v;
   __syncthreads();
 #pragma unroll
-  for (int i = 0; i < Shape<P>::kRunWarps; ++i) v = fmaxf(v, red[first + i]);
+  for (int i = 0; i < kRunWarps; ++i) v = fmaxf(v, red[first + i]);
   return v;
 }
 
@@ -48,114 +92,135 @@ __device__ __forceinline__ float run_max(float v, float* red) {
 // held tokens.  Non-finite inputs do not set the scale: an infinity saturates, NaN becomes 0.
 // Each new value is read once and kept in registers between the maximum and the rounding.
 template <int kKind, int P>
-__global__ void __launch_bounds__(Shape<P>::kThreads)
+__global__ void __launch_bounds__(Shape<P, kAppendRows>::kThreads)
 kv8_append_kernel(const __nv_bfloat16* __restrict__ Kn, int64_t ldk, const __nv_bfloat16* __restrict__ Vn,
                   int64_t ldv, uint8_t* codes, float* scales, float* sums,
                   const int32_t* __restrict__ table, int64_t width, const int32_t* __restrict__ cu,
                   const int32_t* __restrict__ ctx, int64_t T, int max_pages, int Hkv,
                   int64_t num_pages) {
+  using Run = Shape<P, kAppendRows>;
   __shared__ float red[8];
   constexpr float kQ = kv8::code_max<kKind>();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t b = blockIdx.x / max_pages;
-  const int j = blockIdx.x - static_cast<int>(b * max_pages);
-  const int run = blockIdx.y * Shape<P>::kRuns + warp / Shape<P>::kRunWarps;
+  const int b = blockIdx.x / max_pages, j = blockIdx.x - b * max_pages;
+  const int run = blockIdx.y * Run::kRuns + warp / Run::kRunWarps;
   const int side = run >= Hkv, h = run - side * Hkv;
   const int r0 = cu[b], n = cu[b + 1] - r0, len = ctx[b], start = len - n;
-  bool ok = run < 2 * Hkv && n > 0;
   const bool sane = r0 >= 0 && n >= 0 && start >= 0 && r0 + (int64_t)n <= T && (int64_t)len <= width * P;
   const int p = sane ? start / P + j : 0;
-  ok = ok && sane && (int64_t)p * P < len;
-  int64_t page = 0;
-  if (ok) {
-    page = table[b * width + p];
-    if (page < 0 || page >= num_pages) {
-      ok = false;
-      if (threadIdx.x == 0) record(MES_ERR_INVALID);
-    }
-  }
+  bool ok = run < 2 * Hkv && n > 0 && sane && (int64_t)p * P < len;
   if (threadIdx.x == 0 && blockIdx.y == 0) {
     // A sequence with more new tokens than the grid has pages for is an error of the caller.
     if (!sane || (j == 0 && n > 0 && (len - 1) / P - start / P >= max_pages)) record(MES_ERR_INVALID);
   }
-  const __nv_bfloat16* src = side ? Vn : Kn;
+  // The page's slots [old, end) are new; this lane has the even or odd rows of the warp's.
+  const int old = max(start - p * P, 0), end = ok ? min(len - p * P, P) : 0;
+  const int slot0 = warp % Run::kRunWarps * kAppendRows + (lane >> 4), col = (lane & 15) * 8;
   const int64_t ld = side ? ldv : ldk;
-  const int slot0 = warp % Shape<P>::kRunWarps * kWarpRows + (lane >> 4), col = (lane & 15) * 8;
-  uint4 x[8];
-  float amax = 0.f;
+  const __nv_bfloat16* src = (side ? Vn : Kn) + (int64_t)(r0 + p * P + slot0 - start) * ld + h * kv8::kD + col;
+  uint4 x[kAppendRows / 2];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int t = p * P + slot0 + 2 * i;
-    x[i] = make_uint4(0, 0, 0, 0);
-    if (ok && t >= start && t < len)
-      x[i] = __ldg(reinterpret_cast<const uint4*>(src + (int64_t)(r0 + t - start) * ld + h * kv8::kD + col));
+  for (int i = 0; i < kAppendRows / 2; ++i) {
+    const int slot = slot0 + 2 * i;
+    x[i] = slot >= old && slot < end ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
+    src += 2 * ld;
   }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    float f[8];
-    unpack8(x[i], f);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float a = fabsf(f[e]);
-      amax = a <= 3.4028235e38f ? fmaxf(amax, a) : amax;
-    }
+  int64_t page = ok ? table[(int64_t)b * width + p] : 0;
+  if (page < 0 || page >= num_pages) {
+    ok = false;
+    page = 0;
+    record(MES_ERR_INVALID);
   }
   const int64_t si = (page * 2 + side) * Hkv + h;
-  const float was = ok && p * P < start ? scales[si] : 0.f;
-  amax = run_max<P>(amax, red);
+  const float was = ok && old > 0 ? scales[si] : 0.f;
+  // |x| in 16 bits orders as integers do; from 0x7f80 on it is no finite number.
+  uint32_t top = 0;
+#pragma unroll
+  for (int i = 0; i < kAppendRows / 2; ++i)
+    top = __vmaxu2(__vmaxu2(top, __vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu)),
+                   __vmaxu2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu));
+  top = max(top & 0xffffu, top >> 16);
+  const bool odd = top >= 0x7f80u;
+  float amax = __uint_as_float(top << 16);
+  if (odd) {
+    amax = 0.f;
+#pragma unroll
+    for (int i = 0; i < kAppendRows / 2; ++i) {
+      float f[8];
+      unpack8(x[i], f);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) amax = fabsf(f[e]) <= 3.4028235e38f ? fmaxf(amax, fabsf(f[e])) : amax;
+    }
+  }
+  amax = run_max<Run::kRunWarps>(amax, red);
   __syncthreads();                      // every warp of the run has read the old scale
   if (!ok) return;
-  const float now = fmaxf(was, amax / kQ), safe = now > 0.f ? now : 1.f;
-  uint8_t* dst = codes + si * P * kv8::kD;
+  const float now = fmaxf(was, amax / kQ);
+  const Divisor by = divisor(now > 0.f ? now : 1.f, odd);
+  uint8_t* dst = codes + (si * P + slot0) * kv8::kD + col;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const int slot = slot0 + 2 * i, t = p * P + slot;
-    if (t >= len || (t < start && !(now > was))) continue;
-    uint2* at = reinterpret_cast<uint2*>(dst + slot * kv8::kD + col);
-    float f[8];
-    if (t >= start) {
+  for (int i = 0; i < kAppendRows / 2; ++i) {
+    const int slot = slot0 + 2 * i;
+    if (slot >= old && slot < end) {
+      float f[8];
       unpack8(x[i], f);
-    } else {
-      const uint2 old = *at;
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-        f[e] = kv8::decode<kKind>((e < 4 ? old.x : old.y) >> (8 * (e & 3))) * was;
+      *reinterpret_cast<uint2*>(dst + 2 * i * kv8::kD) = quantise8<kKind>(f, by);
     }
-    uint32_t o[2] = {0, 0};
-#pragma unroll
-    for (int e = 0; e < 8; ++e) o[e >> 2] |= kv8::encode<kKind>(f[e] / safe) << (8 * (e & 3));
-    *at = make_uint2(o[0], o[1]);
-    if (sums && side == 0 && t >= start && col == 0) sums[(page * Hkv + h) * P + slot] = 0.f;
   }
-  if (lane == 0 && warp % Shape<P>::kRunWarps == 0) scales[si] = now;
+  if (old > 0 && now > was) {
+    for (int slot = slot0; slot < min(old, slot0 + kAppendRows); slot += 2) {
+      uint2* at = reinterpret_cast<uint2*>(dst + (slot - slot0) * kv8::kD);
+      const uint2 c = *at;
+      float f[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) f[e] = kv8::decode<kKind>((e < 4 ? c.x : c.y) >> (8 * (e & 3))) * was;
+      *at = quantise8<kKind>(f, by);
+    }
+  }
+  if (sums && side == 0 && col == 0)
+    for (int slot = slot0; slot < slot0 + kAppendRows; slot += 2)
+      if (slot >= old && slot < end) sums[(page * Hkv + h) * P + slot] = 0.f;
+  if (lane == 0 && warp % Run::kRunWarps == 0) scales[si] = now;
 }
 
 // ------------------------------------------ read ---------------------------------------
-// out[i] = code * scale of pages[i], rounded to bf16: one 16-byte load and two 16-byte stores a
-// thread.
+// out[i] = code * scale of pages[i], rounded to bf16: four 16-byte loads and eight 16-byte stores a
+// thread, a block for a piece of a page.
+constexpr int kReadChunks = 4;
 template <int kKind>
-__global__ void kv8_read_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ scales,
-                                const int32_t* __restrict__ pages, int64_t chunks, int64_t page_chunks,
-                                int64_t run_chunks, int64_t num_pages, uint4* __restrict__ out) {
-  for (int64_t i = blockIdx.x * (int64_t)blockDim.x + threadIdx.x; i < chunks;
-       i += (int64_t)gridDim.x * blockDim.x) {
-    const int64_t n = i / page_chunks, r = i - n * page_chunks;
-    const int64_t page = __ldg(pages + n);
-    uint4 o[2] = {};
-    if (page < 0 || page >= num_pages) {
-      if (r == 0) record(MES_ERR_INVALID);
-    } else {
-      const uint4 v = __ldg(reinterpret_cast<const uint4*>(codes) + page * page_chunks + r);
-      const float s = __ldg(scales + page * (page_chunks / run_chunks) + r / run_chunks);
-      const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-      uint32_t* u = reinterpret_cast<uint32_t*>(o);
+__global__ void __launch_bounds__(256)
+kv8_read_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ scales,
+                const int32_t* __restrict__ pages, int page_chunks, int run_shift, int64_t num_pages,
+                uint4* __restrict__ out) {
+  const int64_t n = blockIdx.x, page = __ldg(pages + n);
+  const bool ok = page >= 0 && page < num_pages;
+  if (!ok && threadIdx.x == 0) record(MES_ERR_INVALID);
+  const int first = blockIdx.y * kReadChunks * 256 + threadIdx.x;
+  uint4 v[kReadChunks];
+  float s[kReadChunks];
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        u[e] = mes::pack_bf16x2(kv8::decode<kKind>(w[e >> 1] >> (16 * (e & 1))) * s,
-                                kv8::decode<kKind>(w[e >> 1] >> (16 * (e & 1) + 8)) * s);
+  for (int i = 0; i < kReadChunks; ++i) {
+    const int r = first + 256 * i;
+    v[i] = make_uint4(0, 0, 0, 0);
+    s[i] = 0.f;
+    if (ok && r < page_chunks) {
+      v[i] = __ldg(reinterpret_cast<const uint4*>(codes) + page * page_chunks + r);
+      s[i] = __ldg(scales + page * (page_chunks >> run_shift) + (r >> run_shift));
     }
-    out[2 * i] = o[0];
-    out[2 * i + 1] = o[1];
+  }
+#pragma unroll
+  for (int i = 0; i < kReadChunks; ++i) {
+    const int r = first + 256 * i;
+    if (r >= page_chunks) return;
+    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+    uint32_t u[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      u[e] = mes::pack_bf16x2(kv8::decode<kKind>(w[e >> 1] >> (16 * (e & 1))) * s[i],
+                              kv8::decode<kKind>(w[e >> 1] >> (16 * (e & 1) + 8)) * s[i]);
+    uint4* dst = out + 2 * (n * page_chunks + r);
+    dst[0] = make_uint4(u[0], u[1], u[2], u[3]);
+    dst[1] = make_uint4(u[4], u[5], u[6], u[7]);
   }
 }
 
@@ -176,12 +241,17 @@ __device__ __forceinline__ uint32_t order_key(float f) {
 }
 
 struct SelShared {
-  uint32_t hist[kBins];
+  alignas(8) uint32_t hist[kBins];
   uint32_t warp_sum[2][kSelWarps];
   uint32_t digit, above;       // this pass's bin and how many keys lie above it
   uint32_t greater, equal;     // this block's counts against the threshold
 };
 
+__device__ __forceinline__ uint2 ld_dsmem_u32x2(uint32_t addr) {
+  uint2 v;
+  asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ uint32_t ld_dsmem_u32(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
@@ -190,21 +260,21 @@ __device__ __forceinline__ uint32_t ld_dsmem_u32(uint32_t addr) {
 
 __global__ void __launch_bounds__(kSelThreads)
 kv8_select_kernel(const float* __restrict__ sums, const int32_t* __restrict__ table, int64_t width,
-                  const int32_t* __restrict__ ctx, int Hkv, int P, int64_t num_pages, int keep,
+                  const int32_t* __restrict__ ctx, int Hkv, int page_shift, int64_t num_pages, int keep,
                   int recent, int cap, int ranks, int32_t* __restrict__ kept,
                   int32_t* __restrict__ new_lens) {
   extern __shared__ uint32_t cached[];
   __shared__ SelShared sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = ranks > 1 ? static_cast<int>(mes::cluster_ctarank()) : 0;
-  const int64_t item = blockIdx.x / ranks, b = item / Hkv;
-  const int h = static_cast<int>(item - b * Hkv);
+  const int item = blockIdx.x / ranks, b = item / Hkv, h = item - b * Hkv;
+  const int64_t room = width << page_shift;
   int len = ctx[b];
-  if (len < 0 || len > width * P) {
+  if (len < 0 || len > room) {
     if (tid == 0) record(MES_ERR_INVALID);
-    len = len < 0 ? 0 : static_cast<int>(width * P);
+    len = len < 0 ? 0 : static_cast<int>(room);
   }
-  int32_t* out = kept + item * keep;
+  int32_t* out = kept + (int64_t)item * keep;
   const int left = min(len, keep);
   if (h == 0 && rank == 0 && tid == 0) new_lens[b] = left;
   if (len <= keep) {   // nothing to evict (uniform over the cluster)
@@ -220,14 +290,16 @@ kv8_select_kernel(const float* __restrict__ sums, const int32_t* __restrict__ ta
   const int lo = min(rank * slice, n), count = min(lo + slice, n) - lo;
   auto load = [&](int i) {
     const int t = lo + i;
-    int64_t page = table[b * width + t / P];
+    int64_t page = table[b * width + (t >> page_shift)];
     if (page < 0 || page >= num_pages) {
       record(MES_ERR_INVALID);
       page = 0;
     }
-    return order_key(sums[(page * Hkv + h) * P + t % P]);
+    return order_key(sums[((page * Hkv + h) << page_shift) + (t & ((1 << page_shift) - 1))]);
   };
-  for (int i = tid; i < min(count, cap); i += kSelThreads) cached[i] = load(i);
+  const int in_smem = min(count, cap);
+#pragma unroll 8
+  for (int i = tid; i < in_smem; i += kSelThreads) cached[i] = load(i);
   auto key = [&](int i) { return i < cap ? cached[i] : load(i); };
 
   uint32_t prefix = 0, want = k;      // the threshold's high bits; its place among the keys that share them
@@ -247,11 +319,13 @@ kv8_select_kernel(const float* __restrict__ sums, const int32_t* __restrict__ ta
     uint32_t hi = 0, lo2 = 0;
     if (ranks > 1) {
       const uint32_t at = mes::smem_u32(&sh.hist[top - 1]);
-      for (int r = 0; r < ranks; ++r) {
-        const uint32_t a = mes::mapa_shared(at, r);
-        lo2 += ld_dsmem_u32(a);
-        hi += ld_dsmem_u32(a + 4);
-      }
+#pragma unroll
+      for (int r = 0; r < 8; ++r)
+        if (r < ranks) {
+          const uint2 v = ld_dsmem_u32x2(mes::mapa_shared(at, r));
+          lo2 += v.x;
+          hi += v.y;
+        }
     } else {
       hi = sh.hist[top];
       lo2 = sh.hist[top - 1];
@@ -331,32 +405,33 @@ kv8_select_kernel(const float* __restrict__ sums, const int32_t* __restrict__ ta
 // scale is the largest of its sources' scales, so tokens from the source that has it move
 // unchanged and the others are re-rounded once.
 template <int kKind, int P>
-__global__ void __launch_bounds__(Shape<P>::kThreads)
+__global__ void __launch_bounds__(Shape<P, kCompactRows>::kThreads)
 kv8_compact_kernel(uint8_t* codes, float* scales, float* sums, const int32_t* __restrict__ table,
-                   int64_t width, const int32_t* __restrict__ new_table, int64_t new_width,
+                   int64_t width, const int32_t* __restrict__ new_table, int new_width,
                    const int32_t* __restrict__ kept, int keep, int Hkv, int64_t num_pages) {
-  __shared__ float red[8];
+  using Run = Shape<P, kCompactRows>;
+  __shared__ float red[16];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t b = blockIdx.x / new_width, j = blockIdx.x - b * new_width;
-  const int run = blockIdx.y * Shape<P>::kRuns + warp / Shape<P>::kRunWarps;
+  const int b = blockIdx.x / new_width, j = blockIdx.x - b * new_width;
+  const int run = blockIdx.y * Run::kRuns + warp / Run::kRunWarps;
   const int side = run >= Hkv, h = run - side * Hkv;
   bool ok = run < 2 * Hkv;
   int64_t to = 0;
   if (ok) {
-    to = new_table[b * new_width + j];
+    to = new_table[blockIdx.x];
     if (to < 0 || to >= num_pages) {
       ok = false;
       record(MES_ERR_INVALID);
     }
   }
-  // Lane l < 16 looks up token l of the warp's 16 rows.
-  const int slot0 = warp % Shape<P>::kRunWarps * kWarpRows;
-  const int64_t place = j * P + slot0 + (lane & 15);
-  const int t = ok && place < keep ? kept[(b * Hkv + h) * keep + place] : -1;
+  // Lane l < 8 looks up token l of the warp's 8 rows.
+  const int slot0 = warp % Run::kRunWarps * kCompactRows;
+  const int place = j * P + slot0 + (lane & 7);
+  const int t = ok && place < keep ? kept[((int64_t)b * Hkv + h) * keep + place] : -1;
   int64_t row = -1;
   float s = 0.f, sum = 0.f;
   if (t >= 0) {
-    const int64_t page = table[b * width + t / P];
+    const int64_t page = table[(int64_t)b * width + t / P];
     if (page < 0 || page >= num_pages) {
       record(MES_ERR_INVALID);
     } else {
@@ -366,35 +441,37 @@ kv8_compact_kernel(uint8_t* codes, float* scales, float* sums, const int32_t* __
       if (side == 0) sum = sums[(page * Hkv + h) * P + t % P];
     }
   }
-  uint4 v[4];
+  uint4 v[kCompactRows / 4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kCompactRows / 4; ++i) {
     const int64_t r = __shfl_sync(0xffffffffu, row, 4 * i + (lane >> 3));
     v[i] = r >= 0 ? *reinterpret_cast<const uint4*>(codes + r * kv8::kD + (lane & 7) * 16)
                   : make_uint4(0, 0, 0, 0);
   }
-  const float now = run_max<P>(s, red), safe = now > 0.f ? now : 1.f;
+  const float now = run_max<Run::kRunWarps>(s, red);
+  const Divisor by = divisor(now > 0.f ? now : 1.f, false);
   const int64_t di = (to * 2 + side) * Hkv + h;
 #pragma unroll
-  for (int i = 0; i < 4; ++i) {
+  for (int i = 0; i < kCompactRows / 4; ++i) {
     const float was = __shfl_sync(0xffffffffu, s, 4 * i + (lane >> 3));
     if (was != now) {
-      uint32_t* w = reinterpret_cast<uint32_t*>(&v[i]);
+      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
+      uint2 o[2];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        uint32_t o = 0;
+      for (int e = 0; e < 2; ++e) {
+        float f[8];
 #pragma unroll
-        for (int q = 0; q < 4; ++q)
-          o |= kv8::encode<kKind>(kv8::decode<kKind>(w[e] >> (8 * q)) * was / safe) << (8 * q);
-        w[e] = o;
+        for (int q = 0; q < 8; ++q) f[q] = kv8::decode<kKind>(w[2 * e + (q >> 2)] >> (8 * (q & 3))) * was;
+        o[e] = quantise8<kKind>(f, by);
       }
+      v[i] = make_uint4(o[0].x, o[0].y, o[1].x, o[1].y);
     }
     if (ok)
       *reinterpret_cast<uint4*>(codes + (di * P + slot0 + 4 * i + (lane >> 3)) * kv8::kD + (lane & 7) * 16) = v[i];
   }
   if (!ok) return;
-  if (side == 0 && lane < 16) sums[(to * Hkv + h) * P + slot0 + lane] = sum;
-  if (lane == 0 && warp % Shape<P>::kRunWarps == 0) scales[di] = now;
+  if (side == 0 && lane < kCompactRows) sums[(to * Hkv + h) * P + slot0 + lane] = sum;
+  if (lane == 0 && warp % Run::kRunWarps == 0) scales[di] = now;
 }
 
 template <typename F>
@@ -440,9 +517,10 @@ extern "C" int mes_kv8_append(int dtype, const void* K, int64_t ldk, const void*
   if (B * pages > 0x7fffffffll) return MES_ERR_INVALID;
   return by_page(page_size, [&](auto p) {
     constexpr int P = decltype(p)::value;
-    const dim3 grid((unsigned)(B * pages), run_blocks(Hkv, Shape<P>::kRuns));
+    using Run = Shape<P, kAppendRows>;
+    const dim3 grid((unsigned)(B * pages), run_blocks(Hkv, Run::kRuns));
     auto kernel = dtype == kv8::kInt8 ? kv8_append_kernel<kv8::kInt8, P> : kv8_append_kernel<kv8::kE4m3, P>;
-    kernel<<<grid, Shape<P>::kThreads, 0, (cudaStream_t)stream>>>(
+    kernel<<<grid, Run::kThreads, 0, (cudaStream_t)stream>>>(
         (const __nv_bfloat16*)K, ldk, (const __nv_bfloat16*)V, ldv, (uint8_t*)codes, scales, sums,
         block_table, table_width, cu_new, context_lens, T, (int)pages, Hkv, num_pages);
     return mes_host::from_cuda(cudaGetLastError());
@@ -457,13 +535,13 @@ extern "C" int mes_kv8_read(int dtype, const void* codes, const float* scales, c
   if (!codes || !scales || !pages || !out) return MES_ERR_INVALID;
   if (!kv8::aligned(codes, 16) || !kv8::aligned(out, 16) || !kv8::aligned(scales, 4) || !kv8::aligned(pages, 4))
     return MES_ERR_ALIGN;
-  const int64_t run_chunks = (int64_t)page_size * D / 16, page_chunks = run_chunks * 2 * Hkv;
-  if (n > 0x7fffffffffffffffll / (page_chunks * 32)) return MES_ERR_INVALID;
-  const int64_t chunks = n * page_chunks, cap = (int64_t)mes_host::sm_count() * 32;
-  const int64_t blocks = (chunks + 255) / 256;
+  const int run_shift = __builtin_ctz((unsigned)page_size * D / 16);
+  const int page_chunks = (2 * Hkv) << run_shift;
+  if (n > 0x7fffffffll || n > 0x7fffffffffffffffll / ((int64_t)page_chunks * 32)) return MES_ERR_INVALID;
+  const dim3 grid((unsigned)n, (unsigned)((page_chunks + 256 * kReadChunks - 1) / (256 * kReadChunks)));
   auto kernel = dtype == kv8::kInt8 ? kv8_read_kernel<kv8::kInt8> : kv8_read_kernel<kv8::kE4m3>;
-  kernel<<<(unsigned)(blocks < cap ? blocks : cap), 256, 0, (cudaStream_t)stream>>>(
-      (const uint8_t*)codes, scales, pages, chunks, page_chunks, run_chunks, num_pages, (uint4*)out);
+  kernel<<<grid, 256, 0, (cudaStream_t)stream>>>((const uint8_t*)codes, scales, pages, page_chunks, run_shift,
+                                                 num_pages, (uint4*)out);
   return mes_host::from_cuda(cudaGetLastError());
 }
 
@@ -484,10 +562,11 @@ extern "C" int mes_kv8_evict(int dtype, void* codes, float* scales, float* sums,
       !kv8::aligned(block_table, 4) || !kv8::aligned(context_lens, 4) || !kv8::aligned(new_table, 4) ||
       !kv8::aligned(kept, 4) || !kv8::aligned(new_lens, 4))
     return MES_ERR_ALIGN;
-  // Blocks of a cluster: one for each 4096 possible tokens, at most 8 (the portable limit).
+  // Blocks of a cluster, at most 8 (the portable limit): one for each 8192 possible tokens, and one
+  // for each 1024 while that fills SMs.
   const int64_t most = table_width * page_size;
   int ranks = 1;
-  while (ranks < 8 && (int64_t)ranks * 4096 < most) ranks *= 2;
+  while (ranks < 8 && (ranks * 8192ll < most || (ranks * 1024ll < most && B * Hkv * ranks * 2 <= mes_host::sm_count()))) ranks *= 2;
   if (B * Hkv > 0x7fffffffll / ranks || B * new_width > 0x7fffffffll) return MES_ERR_INVALID;
   // Keys kept in shared memory (up to 192 KB); a longer slice's rest is read again in each pass.
   const int64_t slice = (most + ranks - 1) / ranks + 32;
@@ -510,15 +589,16 @@ extern "C" int mes_kv8_evict(int dtype, void* codes, float* scales, float* sums,
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kv8_select_kernel, (const float*)sums, block_table, table_width,
-                                     context_lens, Hkv, page_size, num_pages, (int)keep, (int)recent,
+                                     context_lens, Hkv, __builtin_ctz((unsigned)page_size), num_pages, (int)keep, (int)recent,
                                      cap, ranks, kept, new_lens);
   if (e != cudaSuccess) return MES_ERR_CUDA;
   return by_page(page_size, [&](auto p) {
     constexpr int P = decltype(p)::value;
-    const dim3 grid((unsigned)(B * new_width), run_blocks(Hkv, Shape<P>::kRuns));
+    using Run = Shape<P, kCompactRows>;
+    const dim3 grid((unsigned)(B * new_width), run_blocks(Hkv, Run::kRuns));
     auto kernel = dtype == kv8::kInt8 ? kv8_compact_kernel<kv8::kInt8, P> : kv8_compact_kernel<kv8::kE4m3, P>;
-    kernel<<<grid, Shape<P>::kThreads, 0, (cudaStream_t)stream>>>(
-        (uint8_t*)codes, scales, sums, block_table, table_width, new_table, new_width, kept, (int)keep,
+    kernel<<<grid, Run::kThreads, 0, (cudaStream_t)stream>>>(
+        (uint8_t*)codes, scales, sums, block_table, table_width, new_table, (int)new_width, kept, (int)keep,
         Hkv, num_pages);
     return mes_host::from_cuda(cudaGetLastError());
   });
