@@ -28,10 +28,22 @@ __device__ __forceinline__ uint32_t encode(float x) {
   if (kKind == kInt8) return static_cast<uint32_t>(__float2int_rn(x)) & 0xffu;
   return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
 }
+// The four codes of a word as numbers.  int8: a byte with its sign bit flipped, as the low mantissa of
+// 2^23, is 2^23 + 128 + code (the integer conversion would take the slow unit).
 template <int kKind>
-__device__ __forceinline__ float decode(uint32_t code) {
-  if (kKind == kInt8) return static_cast<float>(static_cast<int8_t>(code & 0xffu));
-  return __half2float(__half(__nv_cvt_fp8_to_halfraw(static_cast<__nv_fp8_storage_t>(code & 0xffu), __NV_E4M3)));
+__device__ __forceinline__ void decode4(uint32_t w, float* f) {
+  if (kKind == kInt8) {
+    const uint32_t u = w ^ 0x80808080u;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) f[e] = __uint_as_float(__byte_perm(u, 0x4b000000u, 0x7650 | e)) - 8388736.f;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float2 t = __half22float2(__half2(__nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(w >> (16 * e)), __NV_E4M3)));
+      f[2 * e] = t.x;
+      f[2 * e + 1] = t.y;
+    }
+  }
 }
 
 // Host checks shared by the entry points.

@@ -64,13 +64,13 @@ __device__ __forceinline__ uint2 quantise8(const float (&f)[8], const Divisor& b
 
 // Rows of one run handled by a warp, and the block shape that follows: a run of P tokens takes
 // P / kRows warps, and a block holds at least four warps, so small pages share a block.
-template <int P, int kRows>
+constexpr int kRows = 16;
+template <int P>
 struct Shape {
   static constexpr int kRunWarps = P / kRows;
   static constexpr int kRuns = kRunWarps < 4 ? 4 / kRunWarps : 1;   // runs of a block
   static constexpr int kThreads = 32 * kRunWarps * kRuns;
 };
-constexpr int kAppendRows = 16, kCompactRows = 8;
 
 // Largest value over the warps of a run; every thread of the block calls it.
 template <int kRunWarps>
@@ -92,13 +92,13 @@ __device__ __forceinline__ float run_max(float v, float* red) {
 // held tokens.  Non-finite inputs do not set the scale: an infinity saturates, NaN becomes 0.
 // Each new value is read once and kept in registers between the maximum and the rounding.
 template <int kKind, int P>
-__global__ void __launch_bounds__(Shape<P, kAppendRows>::kThreads)
+__global__ void __launch_bounds__(Shape<P>::kThreads)
 kv8_append_kernel(const __nv_bfloat16* __restrict__ Kn, int64_t ldk, const __nv_bfloat16* __restrict__ Vn,
                   int64_t ldv, uint8_t* codes, float* scales, float* sums,
                   const int32_t* __restrict__ table, int64_t width, const int32_t* __restrict__ cu,
                   const int32_t* __restrict__ ctx, int64_t T, int max_pages, int Hkv,
                   int64_t num_pages) {
-  using Run = Shape<P, kAppendRows>;
+  using Run = Shape<P>;
   __shared__ float red[8];
   constexpr float kQ = kv8::code_max<kKind>();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -115,12 +115,12 @@ kv8_append_kernel(const __nv_bfloat16* __restrict__ Kn, int64_t ldk, const __nv_
   }
   // The page's slots [old, end) are new; this lane has the even or odd rows of the warp's.
   const int old = max(start - p * P, 0), end = ok ? min(len - p * P, P) : 0;
-  const int slot0 = warp % Run::kRunWarps * kAppendRows + (lane >> 4), col = (lane & 15) * 8;
+  const int slot0 = warp % Run::kRunWarps * kRows + (lane >> 4), col = (lane & 15) * 8;
   const int64_t ld = side ? ldv : ldk;
   const __nv_bfloat16* src = (side ? Vn : Kn) + (int64_t)(r0 + p * P + slot0 - start) * ld + h * kv8::kD + col;
-  uint4 x[kAppendRows / 2];
+  uint4 x[kRows / 2];
 #pragma unroll
-  for (int i = 0; i < kAppendRows / 2; ++i) {
+  for (int i = 0; i < kRows / 2; ++i) {
     const int slot = slot0 + 2 * i;
     x[i] = slot >= old && slot < end ? __ldg(reinterpret_cast<const uint4*>(src)) : make_uint4(0, 0, 0, 0);
     src += 2 * ld;
@@ -136,7 +136,7 @@ kv8_append_kernel(const __nv_bfloat16* __restrict__ Kn, int64_t ldk, const __nv_
   // |x| in 16 bits orders as integers do; from 0x7f80 on it is no finite number.
   uint32_t top = 0;
 #pragma unroll
-  for (int i = 0; i < kAppendRows / 2; ++i)
+  for (int i = 0; i < kRows / 2; ++i)
     top = __vmaxu2(__vmaxu2(top, __vmaxu2(x[i].x & 0x7fff7fffu, x[i].y & 0x7fff7fffu)),
                    __vmaxu2(x[i].z & 0x7fff7fffu, x[i].w & 0x7fff7fffu));
   top = max(top & 0xffffu, top >> 16);
@@ -145,7 +145,7 @@ kv8_append_kernel(const __nv_bfloat16* __restrict__ Kn, int64_t ldk, const __nv_
   if (odd) {
     amax = 0.f;
 #pragma unroll
-    for (int i = 0; i < kAppendRows / 2; ++i) {
+    for (int i = 0; i < kRows / 2; ++i) {
       float f[8];
       unpack8(x[i], f);
 #pragma unroll
@@ -159,7 +159,7 @@ kv8_append_kernel(const __nv_bfloat16* __restrict__ Kn, int64_t ldk, const __nv_
   const Divisor by = divisor(now > 0.f ? now : 1.f, odd);
   uint8_t* dst = codes + (si * P + slot0) * kv8::kD + col;
 #pragma unroll
-  for (int i = 0; i < kAppendRows / 2; ++i) {
+  for (int i = 0; i < kRows / 2; ++i) {
     const int slot = slot0 + 2 * i;
     if (slot >= old && slot < end) {
       float f[8];
@@ -168,17 +168,19 @@ kv8_append_kernel(const __nv_bfloat16* __restrict__ Kn, int64_t ldk, const __nv_
     }
   }
   if (old > 0 && now > was) {
-    for (int slot = slot0; slot < min(old, slot0 + kAppendRows); slot += 2) {
+    for (int slot = slot0; slot < min(old, slot0 + kRows); slot += 2) {
       uint2* at = reinterpret_cast<uint2*>(dst + (slot - slot0) * kv8::kD);
       const uint2 c = *at;
       float f[8];
+      kv8::decode4<kKind>(c.x, f);
+      kv8::decode4<kKind>(c.y, f + 4);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] = kv8::decode<kKind>((e < 4 ? c.x : c.y) >> (8 * (e & 3))) * was;
+      for (int e = 0; e < 8; ++e) f[e] *= was;
       *at = quantise8<kKind>(f, by);
     }
   }
   if (sums && side == 0 && col == 0)
-    for (int slot = slot0; slot < slot0 + kAppendRows; slot += 2)
+    for (int slot = slot0; slot < slot0 + kRows; slot += 2)
       if (slot >= old && slot < end) sums[(page * Hkv + h) * P + slot] = 0.f;
   if (lane == 0 && warp % Run::kRunWarps == 0) scales[si] = now;
 }
@@ -215,9 +217,12 @@ kv8_read_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ sca
     const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
     uint32_t u[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
-      u[e] = mes::pack_bf16x2(kv8::decode<kKind>(w[e >> 1] >> (16 * (e & 1))) * s[i],
-                              kv8::decode<kKind>(w[e >> 1] >> (16 * (e & 1) + 8)) * s[i]);
+    for (int e = 0; e < 4; ++e) {
+      float f[4];
+      kv8::decode4<kKind>(w[e], f);
+      u[2 * e] = mes::pack_bf16x2(f[0] * s[i], f[1] * s[i]);
+      u[2 * e + 1] = mes::pack_bf16x2(f[2] * s[i], f[3] * s[i]);
+    }
     uint4* dst = out + 2 * (n * page_chunks + r);
     dst[0] = make_uint4(u[0], u[1], u[2], u[3]);
     dst[1] = make_uint4(u[4], u[5], u[6], u[7]);
@@ -244,7 +249,8 @@ struct SelShared {
   alignas(8) uint32_t hist[kBins];
   uint32_t warp_sum[2][kSelWarps];
   uint32_t digit, above;       // this pass's bin and how many keys lie above it
-  uint32_t greater, equal;     // this block's counts against the threshold
+  alignas(8) uint32_t greater;
+  uint32_t equal;              // this block's counts against the threshold
 };
 
 __device__ __forceinline__ uint2 ld_dsmem_u32x2(uint32_t addr) {
@@ -252,18 +258,12 @@ __device__ __forceinline__ uint2 ld_dsmem_u32x2(uint32_t addr) {
   asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ uint32_t ld_dsmem_u32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
-}
-
 __global__ void __launch_bounds__(kSelThreads)
 kv8_select_kernel(const float* __restrict__ sums, const int32_t* __restrict__ table, int64_t width,
                   const int32_t* __restrict__ ctx, int Hkv, int page_shift, int64_t num_pages, int keep,
-                  int recent, int cap, int ranks, int32_t* __restrict__ kept,
+                  int recent, int cap, int ranks, bool vectors, int32_t* __restrict__ kept,
                   int32_t* __restrict__ new_lens) {
-  extern __shared__ uint32_t cached[];
+  extern __shared__ __align__(16) uint32_t cached[];
   __shared__ SelShared sh;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = ranks > 1 ? static_cast<int>(mes::cluster_ctarank()) : 0;
@@ -285,21 +285,32 @@ kv8_select_kernel(const float* __restrict__ sums, const int32_t* __restrict__ ta
   const uint32_t k = static_cast<uint32_t>(keep - recent);
   for (int i = rank * kSelThreads + tid; i < recent; i += ranks * kSelThreads) out[k + i] = n + i;
   if (k == 0) return;
-  // Slices are multiples of 32 tokens.
+  // Slices are multiples of 32 tokens, so four tokens at a multiple of 4 lie in one page; what a
+  // last four reads past `count` is memory of its page and is not used.
   const int slice = ((n + ranks - 1) / ranks + 31) / 32 * 32;
   const int lo = min(rank * slice, n), count = min(lo + slice, n) - lo;
-  auto load = [&](int i) {
+  auto place = [&](int i) {
     const int t = lo + i;
     int64_t page = table[b * width + (t >> page_shift)];
     if (page < 0 || page >= num_pages) {
       record(MES_ERR_INVALID);
       page = 0;
     }
-    return order_key(sums[((page * Hkv + h) << page_shift) + (t & ((1 << page_shift) - 1))]);
+    return sums + ((page * Hkv + h) << page_shift) + (t & ((1 << page_shift) - 1));
   };
   const int in_smem = min(count, cap);
-#pragma unroll 8
-  for (int i = tid; i < in_smem; i += kSelThreads) cached[i] = load(i);
+#pragma unroll 4
+  for (int i = 4 * tid; i < in_smem; i += 4 * kSelThreads) {
+    const float* at = place(i);
+    if (vectors) {
+      const float4 v = *reinterpret_cast<const float4*>(at);
+      *reinterpret_cast<uint4*>(cached + i) = make_uint4(order_key(v.x), order_key(v.y), order_key(v.z), order_key(v.w));
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) cached[i + e] = order_key(at[e]);
+    }
+  }
+  auto load = [&](int i) { return order_key(*place(i)); };
   auto key = [&](int i) { return i < cap ? cached[i] : load(i); };
 
   uint32_t prefix = 0, want = k;      // the threshold's high bits; its place among the keys that share them
@@ -309,6 +320,7 @@ kv8_select_kernel(const float* __restrict__ sums, const int32_t* __restrict__ ta
     const uint32_t mask = (1u << bits[pass]) - 1, high = pass == 0 ? 0u : ~((1u << shifts[pass - 1]) - 1);
     for (int i = tid; i < kBins; i += kSelThreads) sh.hist[i] = 0;
     __syncthreads();
+#pragma unroll 4
     for (int i = tid; i < count; i += kSelThreads) {
       const uint32_t x = key(i);
       if ((x & high) == prefix) atomicAdd(&sh.hist[(x >> shift) & mask], 1u);
@@ -338,9 +350,8 @@ kv8_select_kernel(const float* __restrict__ sums, const int32_t* __restrict__ ta
     }
     if (lane == 31) sh.warp_sum[0][warp] = x;
     __syncthreads();
-    uint32_t before = 0;
-    for (int w = 0; w < warp; ++w) before += sh.warp_sum[0][w];
-    before += x - hi - lo2;          // keys in bins above this thread's
+    // Keys in bins above this thread's.
+    const uint32_t before = __reduce_add_sync(0xffffffffu, lane < warp ? sh.warp_sum[0][lane] : 0u) + x - hi - lo2;
     if (before < want && before + hi >= want) {
       sh.digit = top;
       sh.above = before;
@@ -356,6 +367,7 @@ kv8_select_kernel(const float* __restrict__ sums, const int32_t* __restrict__ ta
   const int per_warp = (slice / 32 + kSelWarps - 1) / kSelWarps * 32;
   const int w0 = min(warp * per_warp, count), w1 = min(w0 + per_warp, count);
   uint32_t gt = 0, eq = 0;
+#pragma unroll 4
   for (int i = w0 + lane; i < w1; i += 32) {
     const uint32_t x = key(i);
     gt += x > prefix;
@@ -368,25 +380,20 @@ kv8_select_kernel(const float* __restrict__ sums, const int32_t* __restrict__ ta
     sh.warp_sum[1][warp] = eq;
   }
   __syncthreads();
-  if (tid == 0) {
-    uint32_t a = 0, e = 0;
-    for (int w = 0; w < kSelWarps; ++w) {
-      a += sh.warp_sum[0][w];
-      e += sh.warp_sum[1][w];
+  if (warp == 0) {
+    const uint32_t a = __reduce_add_sync(0xffffffffu, sh.warp_sum[0][lane]);
+    const uint32_t e = __reduce_add_sync(0xffffffffu, sh.warp_sum[1][lane]);
+    if (lane == 0) {
+      sh.greater = a;
+      sh.equal = e;
     }
-    sh.greater = a;
-    sh.equal = e;
   }
   if (ranks > 1) mes::cluster_sync(); else __syncthreads();
-  uint32_t gt_before = 0, eq_before = 0;
-  for (int r = 0; r < rank; ++r) {
-    gt_before += ld_dsmem_u32(mes::mapa_shared(mes::smem_u32(&sh.greater), r));
-    eq_before += ld_dsmem_u32(mes::mapa_shared(mes::smem_u32(&sh.equal), r));
-  }
-  for (int w = 0; w < warp; ++w) {
-    gt_before += sh.warp_sum[0][w];
-    eq_before += sh.warp_sum[1][w];
-  }
+  uint2 others = make_uint2(0, 0);      // lane r: what block r < rank keeps
+  if (lane < rank) others = ld_dsmem_u32x2(mes::mapa_shared(mes::smem_u32(&sh.greater), lane));
+  uint32_t gt_before = __reduce_add_sync(0xffffffffu, others.x + (lane < warp ? sh.warp_sum[0][lane] : 0u));
+  uint32_t eq_before = __reduce_add_sync(0xffffffffu, others.y + (lane < warp ? sh.warp_sum[1][lane] : 0u));
+#pragma unroll 4
   for (int i0 = w0; i0 < w1; i0 += 32) {
     const int i = i0 + lane;
     const uint32_t x = i < w1 ? key(i) : 0u;
@@ -405,12 +412,12 @@ kv8_select_kernel(const float* __restrict__ sums, const int32_t* __restrict__ ta
 // scale is the largest of its sources' scales, so tokens from the source that has it move
 // unchanged and the others are re-rounded once.
 template <int kKind, int P>
-__global__ void __launch_bounds__(Shape<P, kCompactRows>::kThreads)
+__global__ void __launch_bounds__(Shape<P>::kThreads)
 kv8_compact_kernel(uint8_t* codes, float* scales, float* sums, const int32_t* __restrict__ table,
                    int64_t width, const int32_t* __restrict__ new_table, int new_width,
                    const int32_t* __restrict__ kept, int keep, int Hkv, int64_t num_pages) {
-  using Run = Shape<P, kCompactRows>;
-  __shared__ float red[16];
+  using Run = Shape<P>;
+  __shared__ float red[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.x / new_width, j = blockIdx.x - b * new_width;
   const int run = blockIdx.y * Run::kRuns + warp / Run::kRunWarps;
@@ -424,9 +431,9 @@ kv8_compact_kernel(uint8_t* codes, float* scales, float* sums, const int32_t* __
       record(MES_ERR_INVALID);
     }
   }
-  // Lane l < 8 looks up token l of the warp's 8 rows.
-  const int slot0 = warp % Run::kRunWarps * kCompactRows;
-  const int place = j * P + slot0 + (lane & 7);
+  // Lane l looks up token l of the warp's rows (the upper lanes once more).
+  const int slot0 = warp % Run::kRunWarps * kRows;
+  const int place = j * P + slot0 + (lane & (kRows - 1));
   const int t = ok && place < keep ? kept[((int64_t)b * Hkv + h) * keep + place] : -1;
   int64_t row = -1;
   float s = 0.f, sum = 0.f;
@@ -441,9 +448,9 @@ kv8_compact_kernel(uint8_t* codes, float* scales, float* sums, const int32_t* __
       if (side == 0) sum = sums[(page * Hkv + h) * P + t % P];
     }
   }
-  uint4 v[kCompactRows / 4];
+  uint4 v[kRows / 4];
 #pragma unroll
-  for (int i = 0; i < kCompactRows / 4; ++i) {
+  for (int i = 0; i < kRows / 4; ++i) {
     const int64_t r = __shfl_sync(0xffffffffu, row, 4 * i + (lane >> 3));
     v[i] = r >= 0 ? *reinterpret_cast<const uint4*>(codes + r * kv8::kD + (lane & 7) * 16)
                   : make_uint4(0, 0, 0, 0);
@@ -452,7 +459,7 @@ kv8_compact_kernel(uint8_t* codes, float* scales, float* sums, const int32_t* __
   const Divisor by = divisor(now > 0.f ? now : 1.f, false);
   const int64_t di = (to * 2 + side) * Hkv + h;
 #pragma unroll
-  for (int i = 0; i < kCompactRows / 4; ++i) {
+  for (int i = 0; i < kRows / 4; ++i) {
     const float was = __shfl_sync(0xffffffffu, s, 4 * i + (lane >> 3));
     if (was != now) {
       const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
@@ -460,8 +467,10 @@ kv8_compact_kernel(uint8_t* codes, float* scales, float* sums, const int32_t* __
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         float f[8];
+        kv8::decode4<kKind>(w[2 * e], f);
+        kv8::decode4<kKind>(w[2 * e + 1], f + 4);
 #pragma unroll
-        for (int q = 0; q < 8; ++q) f[q] = kv8::decode<kKind>(w[2 * e + (q >> 2)] >> (8 * (q & 3))) * was;
+        for (int q = 0; q < 8; ++q) f[q] *= was;
         o[e] = quantise8<kKind>(f, by);
       }
       v[i] = make_uint4(o[0].x, o[0].y, o[1].x, o[1].y);
@@ -470,7 +479,7 @@ kv8_compact_kernel(uint8_t* codes, float* scales, float* sums, const int32_t* __
       *reinterpret_cast<uint4*>(codes + (di * P + slot0 + 4 * i + (lane >> 3)) * kv8::kD + (lane & 7) * 16) = v[i];
   }
   if (!ok) return;
-  if (side == 0 && lane < kCompactRows) sums[(to * Hkv + h) * P + slot0 + lane] = sum;
+  if (side == 0 && lane < kRows) sums[(to * Hkv + h) * P + slot0 + lane] = sum;
   if (lane == 0 && warp % Run::kRunWarps == 0) scales[di] = now;
 }
 
@@ -517,7 +526,7 @@ extern "C" int mes_kv8_append(int dtype, const void* K, int64_t ldk, const void*
   if (B * pages > 0x7fffffffll) return MES_ERR_INVALID;
   return by_page(page_size, [&](auto p) {
     constexpr int P = decltype(p)::value;
-    using Run = Shape<P, kAppendRows>;
+    using Run = Shape<P>;
     const dim3 grid((unsigned)(B * pages), run_blocks(Hkv, Run::kRuns));
     auto kernel = dtype == kv8::kInt8 ? kv8_append_kernel<kv8::kInt8, P> : kv8_append_kernel<kv8::kE4m3, P>;
     kernel<<<grid, Run::kThreads, 0, (cudaStream_t)stream>>>(
@@ -590,11 +599,11 @@ extern "C" int mes_kv8_evict(int dtype, void* codes, float* scales, float* sums,
   cfg.numAttrs = 1;
   cudaError_t e = cudaLaunchKernelEx(&cfg, kv8_select_kernel, (const float*)sums, block_table, table_width,
                                      context_lens, Hkv, __builtin_ctz((unsigned)page_size), num_pages, (int)keep, (int)recent,
-                                     cap, ranks, kept, new_lens);
+                                     cap, ranks, kv8::aligned(sums, 16), kept, new_lens);
   if (e != cudaSuccess) return MES_ERR_CUDA;
   return by_page(page_size, [&](auto p) {
     constexpr int P = decltype(p)::value;
-    using Run = Shape<P, kCompactRows>;
+    using Run = Shape<P>;
     const dim3 grid((unsigned)(B * new_width), run_blocks(Hkv, Run::kRuns));
     auto kernel = dtype == kv8::kInt8 ? kv8_compact_kernel<kv8::kInt8, P> : kv8_compact_kernel<kv8::kE4m3, P>;
     kernel<<<grid, Run::kThreads, 0, (cudaStream_t)stream>>>(
