@@ -560,7 +560,8 @@ def awq_gemv(x: torch.Tensor, qweight_mes: torch.Tensor, qzeros: torch.Tensor,
     """``x[M, K] @ W[K, N] (+ bias)`` for at most 16 rows: the projections of a token step
     (``mes_awq_gemv``).  The weights are not rounded to bf16 first, as ``awq_gemm`` does."""
     M, N, K = _gemv_args(x, qweight_mes, qzeros, scales, group_size)
-    if bias is not None:
+    if bias is not None and not (bias.dtype is _BF16 and bias.shape == (N,) and bias.get_device() == x.get_device() >= 0
+                                 and bias.is_contiguous()):
         _arg(bias, "bias", x, torch.bfloat16, (N,), contiguous=True)
     if out is None:
         out = torch.empty((M, N), dtype=_BF16, device=x.device)

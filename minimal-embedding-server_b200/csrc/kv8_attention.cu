@@ -9,7 +9,9 @@
 // Work: a (sequence, kv head, row tile) is an item, 128 keys of it a unit.  The units of all items
 // form one line that is cut evenly among the blocks, whatever the lengths are, so no block waits
 // for a long sequence.  An item cut between blocks leaves at most two partial results a block (its
-// first and its last segment), joined by a second kernel.  The lengths stay on the device.
+// first and its last segment), joined by a second kernel.  The lengths stay on the device.  Where
+// no sequence can be long (the table has room for four units at most), items are dealt whole and
+// there is no second kernel: 500 tokens and one query take 7.9 us with the join.
 //
 // A block is four warps.  Each takes 32 keys of a unit for itself: its own ring of TMA tiles
 // (128-byte swizzle, so the 16-byte reads below meet no bank conflict), its own running maximum
@@ -33,6 +35,8 @@ __device__ int g_err_kv8_attention = 0;
 constexpr int kWarps = 4, kThreads = 32 * kWarps, kTile = 32, kUnit = kWarps * kTile;
 constexpr int kStages = 2;
 constexpr int kMaxSeqs = 1024;
+constexpr int kMaxPrefix = 96;      // what the room for three blocks an SM leaves
+constexpr int kWholeUnits = 4;      // most units of an item that is dealt whole
 constexpr int kHalfBytes = kTile * kv8::kD;                 // one side of a stage
 constexpr int kStageBytes = 2 * kHalfBytes;
 // p' is 2^kShift for a tile's largest value when its reference is set, and may grow to 2^kMost: f16
@@ -46,11 +50,15 @@ template <int N>
 struct Smem {
   uint8_t ring[kWarps][kStages][kStageBytes];   // 1024-byte aligned
   union {
-    float4 o[2][N][8][32];                      // two warps' results on their way to the others
+    float4 o[kWarps][4 * N][32];                // halves of the warps' results on their way to others
     uint2 q1[8][32];                            // N == 1: Q fragments on their way to registers
   };
-  uint2 q[N == 1 ? 1 : N][8][32];               // N > 1: Q fragments
-  float2 ml[2][8 * N];                          // reference and sum of the rows of `o`
+  union {
+    uint2 q[N][8][32];                          // N > 1: Q fragments
+    uint4 raw1[8][16];                          // N == 1: the next segment's query rows
+  };
+  uint4 raw[N == 2 ? 16 : 1][N == 2 ? 16 : 1];  // N == 2: the next segment's query rows
+  float2 ml[kWarps][8 * N];                     // reference and sum of the warps' rows
   float qscale[8 * N];                          // logit factor of a row, in the exp2 domain
   int last[8 * N];                              // last visible key of a row
   float2 sc[kWarps][kStages][3];                // factors of a tile's two halves: K scale, log2 and
@@ -58,10 +66,8 @@ struct Smem {
   uint64_t full[kWarps][kStages];
   int warp_sum[kWarps];
   int abort;
-  int prefix[1];                                // [B + 1]
+  int prefix[kMaxPrefix + 1];                   // units before every `coarse`-th sequence, and all
 };
-template <int N>
-constexpr size_t smem_bytes(int B) { return sizeof(Smem<N>) + 4 * (size_t)B; }
 
 struct Params {
   const __nv_bfloat16* q;
@@ -80,6 +86,7 @@ struct Params {
   float* lse;           // [T * Hq] with sums, else null
   float* logits;        // [T * Hq][max_ctx] with sums, else null
   int64_t max_ctx;
+  int whole;            // units of every item where items are dealt whole, else 0
 };
 
 // Key of an 8-key group that is row n of a product: keys of n and n ^ 1 differ in bit 2, and for a
@@ -101,6 +108,9 @@ __device__ __forceinline__ uint32_t transpose8(uint32_t v) {
   uint32_t r;
   asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
+}
+__device__ __forceinline__ void copy16_async(void* dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(mes::smem_u32(dst)), "l"(src) : "memory");
 }
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int i) {
   return i == 0 ? v.x : i == 1 ? v.y : i == 2 ? v.z : v.w;
@@ -132,9 +142,11 @@ __device__ __forceinline__ void convert(uint32_t w, uint32_t& a, uint32_t& b) {
   b = kKind == kv8::kInt8 ? int8_pair(w >> 8) : e4m3_pair(w >> 16);
 }
 
-// Units of a sequence's items and their number.  A sequence with query rows has at least one unit
-// an item, so that rows that see nothing are written too.
-__device__ __forceinline__ int units_of(int len) { return len > 0 ? (len + kUnit - 1) / kUnit : 1; }
+// Units of an item of a sequence: at least one, so that rows that see nothing are written too; the
+// same for all where items are dealt whole.
+__device__ __forceinline__ int units_of(const Params& p, int len) {
+  return p.whole > 0 ? p.whole : len > 0 ? (len + kUnit - 1) / kUnit : 1;
+}
 template <int N>
 __device__ __forceinline__ int row_tiles(int n, int G) { return (n * G + 8 * N - 1) / (8 * N); }
 
@@ -178,14 +190,15 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
   }
   // The join may be launched as soon as every block of this grid runs (it waits for their end).
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // Units before each sequence.
+  // Units before each sequence, or, of many, every `coarse`-th.
+  const int coarse = (p.B + kMaxPrefix - 1) / kMaxPrefix;
   int total = 0;
   for (int b0 = 0; b0 < p.B; b0 += kThreads) {
     const int b = b0 + tid;
     int x = 0;
     if (b < p.B) {
       const Seq s = sequence(p, b);
-      x = s.n > 0 ? units_of(s.len) * p.Hkv * row_tiles<N>(s.n, p.G) : 0;
+      x = s.n > 0 ? units_of(p, s.len) * p.Hkv * row_tiles<N>(s.n, p.G) : 0;
     }
     const int mine = x;
 #pragma unroll
@@ -198,22 +211,36 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
     __syncthreads();
     int before = total;
     for (int w = 0; w < warp; ++w) before += sh.warp_sum[w];
-    if (b < p.B) sh.prefix[b] = before + x - mine;
+    if (b < p.B && b % coarse == 0) sh.prefix[b / coarse] = before + x - mine;
     for (int w = 0; w < kWarps; ++w) total += sh.warp_sum[w];
   }
-  if (tid == 0) sh.prefix[p.B] = total;
+  const int marks = (p.B + coarse - 1) / coarse;
+  if (tid == 0) sh.prefix[marks] = total;
   __syncthreads();
-  const int blocks = min((int)gridDim.x, total);
+  const int grain = p.whole > 0 ? p.whole : 1;     // a multiple of this many units for each block
+  const int blocks = min((int)gridDim.x, total / grain);
   if ((int)blockIdx.x >= blocks) return;
-  const int first = share(total, blockIdx.x, blocks), end = share(total, blockIdx.x + 1, blocks);
+  const int first = share(total / grain, blockIdx.x, blocks) * grain;
+  const int end = share(total / grain, blockIdx.x + 1, blocks) * grain;
 
-  auto find = [&](int u) {      // sequence of unit u: the last b with prefix[b] <= u that has units
-    int lo = 0, hi = p.B;       // prefix[lo] <= u < prefix[hi]
+  struct Found {
+    int b, base;        // sequence of a unit and the units before it
+    Seq s;
+  };
+  auto find = [&](int u) {
+    int lo = 0, hi = marks;     // prefix[lo] <= u < prefix[hi]
     while (hi - lo > 1) {
       const int mid = (lo + hi) >> 1;
       if (sh.prefix[mid] <= u) lo = mid; else hi = mid;
     }
-    return lo;
+    Found f = {lo * coarse, sh.prefix[lo], sequence(p, lo * coarse)};
+    // Past sequences that end before u (those without query rows have no units).
+    while (true) {
+      const int mine = f.s.n > 0 ? units_of(p, f.s.len) * p.Hkv * row_tiles<N>(f.s.n, p.G) : 0;
+      if (f.base + mine > u || f.b + 1 >= p.B) return f;
+      f.base += mine;
+      f.s = sequence(p, ++f.b);
+    }
   };
 
   // ---- the warp's tiles: unit first + i is its tile i ----
@@ -226,9 +253,10 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
     t_ks = make_float2(0.f, 0.f);
     t_vs = make_float2(1.f, 1.f);
     if (u >= end) return;
-    const int b = find(u);
-    const Seq s = sequence(p, b);
-    const int units = units_of(s.len), rest = u - sh.prefix[b], item = rest / units;
+    const Found at = find(u);
+    const int b = at.b;
+    const Seq s = at.s;
+    const int units = units_of(p, s.len), rest = u - at.base, item = rest / units;
     const int t0 = (rest - item * units) * kUnit + warp * kTile;
     const int h = item / row_tiles<N>(s.n, p.G);
     int64_t page[2] = {0, 0};
@@ -291,30 +319,68 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
       sh.sc[warp][i % kStages][2] = t_iv;
     }
   };
+  // ---- segments: the units of one item that this block has ----
+  struct Segment {
+    int h, row_base, rows, item0, units, stop;
+    Seq s;
+  };
+  auto segment = [&](int u) {
+    Segment g;
+    const Found at = find(u);
+    g.s = at.s;
+    g.units = units_of(p, g.s.len);
+    const int tiles = row_tiles<N>(g.s.n, p.G), rest = u - at.base, item = rest / g.units;
+    g.h = item / tiles;
+    g.row_base = (item - g.h * tiles) * kRows;
+    g.rows = min(kRows, g.s.n * p.G - g.row_base);
+    g.item0 = u - (rest - item * g.units);
+    g.stop = min(end, g.item0 + g.units);
+    return g;
+  };
+  // A thread has sixteen values of a query row (of N / 2 rows for N == 4).
+  auto q_source = [&](const Segment& g, int e) {
+    const int q = g.row_base + (e >> 3), i = q / p.G;
+    return p.q + (int64_t)(g.s.r0 + i) * p.ldq + (g.h * p.G + q - i * p.G) * kv8::kD + (e & 7) * 16;
+  };
+  // Copies the rows of a segment in, while the one before is worked on (32 rows have no room).
+  auto q_ahead = [&](const Segment& g) {
+    if (N > 2) return;
+    for (int e = tid; e < kRows * 8; e += kThreads)
+      if ((e >> 3) < g.rows) {
+        uint4* dst = (N == 1 ? sh.raw1[e >> 3] : sh.raw[e >> 3]) + 2 * (e & 7);
+        const __nv_bfloat16* src = q_source(g, e);
+        copy16_async(dst, src);
+        copy16_async(dst + 1, src + 8);
+      }
+  };
   for (int i = 0; i < kStages; ++i) issue(i);
+  Segment seg = segment(first);
+  q_ahead(seg);
 
   uint32_t phase = 0;           // bit s: parity of stage s's next load
   bool ok = true;
   for (int u = first; u < end;) {
-    // ---- segment: units [u, stop) of one item ----
-    const int b = find(u);
-    const Seq s = sequence(p, b);
-    const int units = units_of(s.len), tiles = row_tiles<N>(s.n, p.G);
-    const int rest = u - sh.prefix[b], item = rest / units, unit0 = rest - item * units;
-    const int h = item / tiles, tile = item - h * tiles;
-    const int item0 = u - unit0, stop = min(end, item0 + units);
-    const int row_base = tile * kRows, rows = min(kRows, s.n * p.G - row_base);
-    const int start = s.len - s.n;
+    const Seq s = seg.s;
+    const int h = seg.h, row_base = seg.row_base, rows = seg.rows, item0 = seg.item0, units = seg.units, stop = seg.stop;
+    const int unit0 = u - item0, start = s.len - s.n;
+    if (N <= 2) asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();            // the previous segment's readers of q / o are done
     // Query rows: f16 times a power of two that brings the row's largest value near 2^8.
     for (int e = tid; e < kRows * 8; e += kThreads) {
-      const int r = e >> 3, part = e & 7, row = row_base + r;
+      const int r = e >> 3, part = e & 7;
       float f[16];
       float amax = 0.f;
       if (r < rows) {
-        const int i = row / p.G, head = h * p.G + row - i * p.G;
-        const uint4* src = reinterpret_cast<const uint4*>(p.q + (int64_t)(s.r0 + i) * p.ldq + head * kv8::kD + part * 16);
-        const uint4 v[2] = {__ldg(src), __ldg(src + 1)};
+        uint4 v[2];
+        if (N <= 2) {
+          const uint4* src = (N == 1 ? sh.raw1[r] : sh.raw[r]) + 2 * part;
+          v[0] = src[0];
+          v[1] = src[1];
+        } else {
+          const uint4* src = reinterpret_cast<const uint4*>(q_source(seg, e));
+          v[0] = __ldg(src);
+          v[1] = __ldg(src + 1);
+        }
         const __nv_bfloat162* hv = reinterpret_cast<const __nv_bfloat162*>(v);
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
@@ -323,7 +389,7 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
           f[2 * j + 1] = t.y;
           amax = fmaxf(amax, fmaxf(fabsf(t.x), fabsf(t.y)));
         }
-        if (part == 0) sh.last[r] = start + i;
+        if (part == 0) sh.last[r] = start + (row_base + r) / p.G;
       } else {
 #pragma unroll
         for (int j = 0; j < 16; ++j) f[j] = 0.f;
@@ -346,6 +412,10 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
       }
     }
     __syncthreads();
+    if (stop < end) {
+      seg = segment(stop);
+      q_ahead(seg);
+    }
     // This lane's rows are 8 t + 2 c + e of tile t.
     float qs[N][2];
     int last[N][2];
@@ -554,84 +624,114 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
       issue(i + kStages);
     }
 
-    // ---- join the four warps: 2 and 3 hand theirs to 0 and 1, then 1 to 0 ----
+    // ---- join the four warps: they trade halves of their sums two apart, then halves of those with
+    // their neighbours, so that warp w ends with the w-th quarter of all ----
 #pragma unroll
     for (int t = 0; t < N; ++t)
 #pragma unroll
       for (int e = 0; e < 2; ++e)
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) l[t][e] += __shfl_xor_sync(0xffffffffu, l[t][e], o);
+    // Element i: tile i / 8, values 2 (i % 8) and one more of its 16.
+    float4 part[4 * N];
+    float mine[N][2], theirs[N][2];
+    auto give_rows = [&] {
+      if (g == 0)
 #pragma unroll
-    for (int from = 2; from > 0; --from) {        // warps [from, 2 from) give, [0, from) take
-      __syncthreads();
-      if (warp >= from && warp < 2 * from) {
+        for (int t = 0; t < N; ++t)
 #pragma unroll
-        for (int t = 0; t < N; ++t) {
-#pragma unroll
-          for (int d = 0; d < 8; ++d)
-            sh.o[warp - from][t][d][lane] = make_float4(O[t][d][0], O[t][d][1], O[t][d][2], O[t][d][3]);
-          if (g == 0) {
-            sh.ml[warp - from][8 * t + 2 * c] = make_float2(m[t][0], l[t][0]);
-            sh.ml[warp - from][8 * t + 2 * c + 1] = make_float2(m[t][1], l[t][1]);
-          }
-        }
-      }
-      __syncthreads();
-      if (warp < from) {
-#pragma unroll
-        for (int t = 0; t < N; ++t) {
-          float mine[2], theirs[2];
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const float2 ml = sh.ml[warp][8 * t + 2 * c + e];
-            const float now = fmaxf(m[t][e], ml.x);
-            mine[e] = m[t][e] == -INFINITY ? 0.f : ex2(m[t][e] - now);
-            theirs[e] = ml.x == -INFINITY ? 0.f : ex2(ml.x - now);
-            m[t][e] = now;
-            l[t][e] = l[t][e] * mine[e] + ml.y * theirs[e];
-          }
-#pragma unroll
-          for (int d = 0; d < 8; ++d) {
-            const float4 x = sh.o[warp][t][d][lane];
-            O[t][d][0] = O[t][d][0] * mine[0] + x.x * theirs[0];
-            O[t][d][1] = O[t][d][1] * mine[1] + x.y * theirs[1];
-            O[t][d][2] = O[t][d][2] * mine[0] + x.z * theirs[0];
-            O[t][d][3] = O[t][d][3] * mine[1] + x.w * theirs[1];
-          }
-        }
-      }
-    }
-    if (warp == 0) {
-      const bool whole = unit0 == 0 && stop == item0 + units;
-      const int slot = 2 * blockIdx.x + (item0 + unit0 == first ? 0 : 1);
+          for (int e = 0; e < 2; ++e) sh.ml[warp][8 * t + 2 * c + e] = make_float2(m[t][e], l[t][e]);
+    };
+    auto take_rows = [&](int from) {     // joins another warp's references and sums
 #pragma unroll
       for (int t = 0; t < N; ++t)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int row = 8 * t + 2 * c + e;
-          if (row >= rows) continue;
-          if (whole) {
-            const int q = row_base + row, qi = q / p.G;
-            const int64_t at = (int64_t)(s.r0 + qi) * p.Hq + h * p.G + q - qi * p.G;
-            const float inv = l[t][e] > 0.f ? 1.f / l[t][e] : l[t][e] == 0.f ? 0.f : l[t][e];      // NaN stays NaN
-            uint4* dst = reinterpret_cast<uint4*>(p.out + at * kv8::kD + 16 * g);
-#pragma unroll
-            for (int q4 = 0; q4 < 2; ++q4) {
-              uint32_t w[4];
-#pragma unroll
-              for (int d = 0; d < 4; ++d)
-                w[d] = mes::pack_bf16x2(O[t][4 * q4 + d][e] * inv, O[t][4 * q4 + d][2 + e] * inv);
-              dst[q4] = make_uint4(w[0], w[1], w[2], w[3]);
-            }
-            if (kSums && g == 0) p.lse[at] = m[t][e] + log2f(l[t][e]);
-          } else {
-            float4* dst = reinterpret_cast<float4*>(p.part_o + ((int64_t)slot * kRows + row) * kv8::kD + 16 * g);
-#pragma unroll
-            for (int q4 = 0; q4 < 4; ++q4)
-              dst[q4] = make_float4(O[t][2 * q4][e], O[t][2 * q4][2 + e], O[t][2 * q4 + 1][e], O[t][2 * q4 + 1][2 + e]);
-            if (g == 0) p.part_ml[(int64_t)slot * kRows + row] = make_float2(m[t][e], l[t][e]);
-          }
+          const float2 ml = sh.ml[from][8 * t + 2 * c + e];
+          const float now = fmaxf(m[t][e], ml.x);
+          mine[t][e] = m[t][e] == -INFINITY ? 0.f : ex2(m[t][e] - now);
+          theirs[t][e] = ml.x == -INFINITY ? 0.f : ex2(ml.x - now);
+          m[t][e] = now;
+          l[t][e] = l[t][e] * mine[t][e] + ml.y * theirs[t][e];
         }
+    };
+    auto join = [&](float4& a, const float4& x, const float (&fm)[2], const float (&ft)[2]) {
+      a.x = a.x * fm[0] + x.x * ft[0];
+      a.y = a.y * fm[1] + x.y * ft[1];
+      a.z = a.z * fm[0] + x.z * ft[0];
+      a.w = a.w * fm[1] + x.w * ft[1];
+    };
+    const bool upper = warp >= 2, odd = warp & 1;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 4 * N; ++i) {
+      const int j = i + 4 * N;
+      const float4 a = make_float4(O[i / 8][i % 8][0], O[i / 8][i % 8][1], O[i / 8][i % 8][2], O[i / 8][i % 8][3]);
+      const float4 z = make_float4(O[j / 8][j % 8][0], O[j / 8][j % 8][1], O[j / 8][j % 8][2], O[j / 8][j % 8][3]);
+      part[i] = upper ? z : a;
+      sh.o[warp][i][lane] = upper ? a : z;
+    }
+    give_rows();
+    __syncthreads();
+    take_rows(warp ^ 2);
+#pragma unroll
+    for (int i = 0; i < 4 * N; ++i) {
+      const int t0 = i / 8, t1 = (i + 4 * N) / 8;
+      const float fm[2] = {upper ? mine[t1][0] : mine[t0][0], upper ? mine[t1][1] : mine[t0][1]};
+      const float ft[2] = {upper ? theirs[t1][0] : theirs[t0][0], upper ? theirs[t1][1] : theirs[t0][1]};
+      join(part[i], sh.o[warp ^ 2][i][lane], fm, ft);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 2 * N; ++i) {
+      sh.o[warp][i][lane] = odd ? part[i] : part[i + 2 * N];
+      part[i] = odd ? part[i + 2 * N] : part[i];
+    }
+    give_rows();
+    __syncthreads();
+    take_rows(warp ^ 1);
+    // This warp's tile and the place of its 4 N values in a lane's 16.
+    const int tile = N == 1 ? 0 : warp * N / 4, at16 = N == 1 ? 4 * warp : N == 2 ? 8 * (warp & 1) : 0;
+    float fm[2] = {0.f, 0.f}, ft[2] = {0.f, 0.f}, row_m[2] = {0.f, 0.f}, row_l[2] = {0.f, 0.f};
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+      if (t == tile)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          fm[e] = mine[t][e];
+          ft[e] = theirs[t][e];
+          row_m[e] = m[t][e];
+          row_l[e] = l[t][e];
+        }
+#pragma unroll
+    for (int i = 0; i < 2 * N; ++i) join(part[i], sh.o[warp ^ 1][i][lane], fm, ft);
+
+    const bool whole = unit0 == 0 && stop == item0 + units;
+    const int slot = 2 * blockIdx.x + (item0 + unit0 == first ? 0 : 1);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int row = 8 * tile + 2 * c + e;
+      if (row >= rows) continue;
+      if (whole) {
+        const int q = row_base + row, qi = q / p.G;
+        const int64_t at = (int64_t)(s.r0 + qi) * p.Hq + h * p.G + q - qi * p.G;
+        const float inv = row_l[e] > 0.f ? 1.f / row_l[e] : row_l[e] == 0.f ? 0.f : row_l[e];      // NaN stays NaN
+        uint32_t w[2 * N];
+#pragma unroll
+        for (int i = 0; i < 2 * N; ++i)
+          w[i] = mes::pack_bf16x2((e ? part[i].y : part[i].x) * inv, (e ? part[i].w : part[i].z) * inv);
+        uint2* dst = reinterpret_cast<uint2*>(p.out + at * kv8::kD + 16 * g + at16);
+#pragma unroll
+        for (int i = 0; i < N; ++i) dst[i] = make_uint2(w[2 * i], w[2 * i + 1]);
+        if (kSums && g == 0 && at16 == 0) p.lse[at] = row_m[e] + log2f(row_l[e]);
+      } else {
+        float4* dst = reinterpret_cast<float4*>(p.part_o + ((int64_t)slot * kRows + row) * kv8::kD + 16 * g + at16);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+          dst[i] = e ? make_float4(part[2 * i].y, part[2 * i].w, part[2 * i + 1].y, part[2 * i + 1].w)
+                     : make_float4(part[2 * i].x, part[2 * i].z, part[2 * i + 1].x, part[2 * i + 1].z);
+        if (g == 0 && at16 == 0) p.part_ml[(int64_t)slot * kRows + row] = make_float2(row_m[e], row_l[e]);
+      }
     }
   }
   if (!ok) {
@@ -662,7 +762,7 @@ kv8_join_kernel(const Params p, int grid) {
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     Seq x = {0, 0, 0};
     if (b0 + lane < p.B) x = sequence(p, b0 + lane);
-    const int mine = x.n > 0 ? units_of(x.len) * p.Hkv * row_tiles<N>(x.n, p.G) : 0;
+    const int mine = x.n > 0 ? units_of(p, x.len) * p.Hkv * row_tiles<N>(x.n, p.G) : 0;
     total += __reduce_add_sync(0xffffffffu, mine);
     before += __reduce_add_sync(0xffffffffu, x.r0 + x.n <= token ? mine : 0);
     const uint32_t found = __ballot_sync(0xffffffffu, x.n > 0 && token >= x.r0 && token < x.r0 + x.n);
@@ -676,7 +776,7 @@ kv8_join_kernel(const Params p, int grid) {
   if (s.n <= 0) return;
   const int blocks = min(grid, total);
   const int row = (token - s.r0) * p.G + head - h * p.G, tile = row / kRows;
-  const int units = units_of(s.len);
+  const int units = units_of(p, s.len);
   const int u0 = before + (h * row_tiles<N>(s.n, p.G) + tile) * units, u1 = u0 + units;
   // The blocks whose shares meet [u0, u1).
   int from = (int)((int64_t)u0 * blocks / total);
@@ -806,13 +906,12 @@ int launch(const CUtensorMap& map, const Params& p, float* sums, void* stream) {
   static std::atomic<uint64_t> configured{0};
   int st = mes_host::once_per_device(configured, [&] {
     return mes_host::from_cuda(
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes<N>(kMaxSeqs)));
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(Smem<N>)));
   });
   if (st != MES_OK) return st;
-  // As many blocks an SM as fit (many sequences take one's place); 1 KB of each is the system's.
-  const int fit = (int)(233472 / (smem_bytes<N>(p.B) + 1024));
-  const int grid = mes_host::persistent_ctas() * (fit < blocks_per_sm(N) ? fit : blocks_per_sm(N));
-  kernel<<<grid, kThreads, smem_bytes<N>(p.B), (cudaStream_t)stream>>>(map, p);
+  static_assert((sizeof(Smem<N>) + 1024) * blocks_per_sm(N) <= 233472, "1 KB of a block is the system's");
+  const int grid = mes_host::persistent_ctas() * blocks_per_sm(N);
+  kernel<<<grid, kThreads, sizeof(Smem<N>), (cudaStream_t)stream>>>(map, p);
   if (cudaGetLastError() != cudaSuccess) return MES_ERR_CUDA;
   // The kernels that follow start while the one before them ends (programmatic launch).
   cudaLaunchAttribute attr = {};
@@ -823,11 +922,12 @@ int launch(const CUtensorMap& map, const Params& p, float* sums, void* stream) {
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
   // Few items leave many partial results each: four warps then share a row's.
-  const bool wide = (int64_t)p.B * p.Hkv * 4 <= grid;
+  const int64_t items = (int64_t)p.Hkv * max(p.B, (p.T * p.G + 8 * N - 1) / (8 * N));
+  const bool wide = items * 4 <= grid;
   const int per_block = wide ? 1 : kWarps;
   cfg.gridDim = dim3((unsigned)(((int64_t)p.T * p.Hq + per_block - 1) / per_block));
   cfg.blockDim = dim3(kThreads);
-  if (cudaLaunchKernelEx(&cfg, wide ? kv8_join_kernel<N, kWarps, kSums> : kv8_join_kernel<N, 1, kSums>, p, grid) != cudaSuccess)
+  if (p.whole == 0 && cudaLaunchKernelEx(&cfg, wide ? kv8_join_kernel<N, kWarps, kSums> : kv8_join_kernel<N, 1, kSums>, p, grid) != cudaSuccess)
     return MES_ERR_CUDA;
   if (kSums) {
     cfg.gridDim = dim3((unsigned)((p.max_ctx + 255) / 256), (unsigned)(p.B * p.Hkv));
@@ -906,6 +1006,8 @@ extern "C" int mes_kv8_attention(int dtype, const void* q, int64_t ldq, const vo
   p.lse = sums ? (float*)(ws + w.lse) : nullptr;
   p.logits = sums ? (float*)(ws + w.logits) : nullptr;
   p.max_ctx = max_ctx;
+  const int64_t most = (table_width * page_size + kUnit - 1) / kUnit;
+  p.whole = most <= kWholeUnits ? (int)most : 0;
   auto go = [&](auto n) {
     constexpr int kN = decltype(n)::value;
     if (dtype == kv8::kInt8)
