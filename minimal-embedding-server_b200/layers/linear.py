@@ -135,6 +135,18 @@ class LinearBase(nn.Module):
                         panel=panel)
         return y.view(*shape[:-1], y.shape[-1])
 
+    # ------------------------------------------------------------------ token steps
+    def _few(self, x: torch.Tensor) -> bool:
+        """Whether ``x [M, K]`` is a token step's: rows for the matrix-vector kernel."""
+        return x.dim() == 2 and 0 < x.shape[0] <= _C.GEMV_MAX_ROWS
+
+    def step(self, x: torch.Tensor) -> torch.Tensor:
+        """``forward`` with the matrix-vector kernel where ``x`` has few enough rows (its weights
+        are not rounded to bf16, so the result may differ from ``forward``'s in the last bits)."""
+        if not self._few(x):
+            return self.forward(x)
+        return _C.awq_gemv(x, *LinearBase.gemm_weights(self), self.bias, group_size=self.group_size)
+
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         raise NotImplementedError
 
@@ -238,6 +250,13 @@ class MergedColumnParallelLinear(ColumnParallelLinear):
         return y.view(*shape[:-1], y.shape[-1])
 
 
+    def step_silu(self, x: torch.Tensor) -> torch.Tensor:
+        """``forward_silu`` for a token step."""
+        if not self._few(x):
+            return self.forward_silu(x)
+        return _C.awq_gemv_silu(x, *self.gemm_weights(), group_size=self.group_size)
+
+
 class QKVParallelLinear(ColumnParallelLinear):
     """``linear.py:110-144``: local output ``[q | k | v]`` with ``num_heads`` and
     ``num_kv_heads`` heads of ``head_size`` per rank."""
@@ -308,4 +327,23 @@ class RowParallelLinear(LinearBase):
         _C.awq_gemm_residual(x.reshape(-1, x.shape[-1]), qw, qz, sc,
                              residual.view(-1, residual.shape[-1]), self.bias,
                              group_size=self.group_size, panel=self.panel)
+        return None
+
+    def step(self, x: torch.Tensor) -> torch.Tensor:
+        if not self._few(x):
+            return self.forward(x)
+        y = _C.awq_gemv(x, *LinearBase.gemm_weights(self), self.bias if self.tp_rank == 0 else None,
+                        group_size=self.group_size)
+        if self.tp_size > 1:
+            dist.all_reduce(y)
+        return y
+
+    def step_residual(self, x: torch.Tensor, residual: torch.Tensor) -> torch.Tensor | None:
+        """``forward_residual`` for a token step."""
+        if not self._few(x):
+            return self.forward_residual(x, residual)
+        if self.tp_size > 1:
+            return self.step(x)
+        _C.awq_gemv_residual(x, *self.gemm_weights(), residual.view(-1, residual.shape[-1]), self.bias,
+                             group_size=self.group_size)
         return None

@@ -16,6 +16,7 @@ the projection was already added.
 """
 from __future__ import annotations
 
+import contextlib
 import os
 
 import torch
@@ -26,6 +27,7 @@ from .. import _C
 from ..layers.activation import SiluAndMul
 from ..layers.attention import batch_schedule, create_attention
 from ..layers.embed_head import VocabParallelEmbedding
+from ..layers.kv_cache import CacheStep, KV8Cache
 from ..layers.layernorm import RMSNorm
 from ..layers.linear import MergedColumnParallelLinear, QKVParallelLinear, RowParallelLinear
 from ..layers.rotary_embedding import get_rope
@@ -103,6 +105,27 @@ class Qwen2Attention(nn.Module):
         return self.o_proj.forward_partial(self._attend(positions, hidden_states))
 
 
+    def step(self, positions: torch.Tensor, hidden_states: torch.Tensor, residual: torch.Tensor,
+             cache: KV8Cache, new: CacheStep, first: bool, seen: tuple | None = None):
+        """Attention block of new tokens whose predecessors are in ``cache``, added into the fp32
+        residual stream.  The new tokens' keys and values are stored first.  ``first``: nothing
+        was cached before, so the tokens attend to one another in 16 bits, as in ``forward``.
+        ``seen``: ``(rows, step)`` of tokens whose attention weights count towards eviction
+        although their output is not needed from the cache."""
+        qkv = self.qkv_proj.step(hidden_states)
+        norms = (self.q_norm, self.k_norm) if self.apply_qk_norm else ()
+        self.rotary_emb.forward_fused(positions, qkv, self.num_heads, self.num_kv_heads, *norms)
+        q, k, v = qkv.split([self.q_size, self.kv_size, self.kv_size], dim=1)
+        cache.append(k, v, new)
+        if first:
+            out = self.attn.forward_packed(qkv, positions)
+            if seen is not None:
+                cache.attend(q.index_select(0, seen[0]), seen[1], self.num_heads, self.scaling)
+        else:
+            out = cache.attend(q, new, self.num_heads, self.scaling)
+        return self.o_proj.step_residual(out, residual)
+
+
 class Qwen2MLP(nn.Module):
 
     def __init__(self, hidden_size: int, intermediate_size: int, hidden_act: str,
@@ -131,6 +154,14 @@ class Qwen2MLP(nn.Module):
     def forward_partial(self, x):
         """This rank's down_proj partial product, before the all-reduce."""
         return self.down_proj.forward_partial(self._act(x))
+
+    def step_residual(self, x, residual):
+        """``forward_residual`` for a token step."""
+        if self.gate_up_proj.supports_silu():
+            act = self.gate_up_proj.step_silu(x)
+        else:
+            act = self.act_fn(self.gate_up_proj.step(x))
+        return self.down_proj.step_residual(act, residual)
 
 
 def _attn_kwargs(model_config, qkv_bias: bool, qk_norm: bool) -> dict:
@@ -227,6 +258,20 @@ class DecoderLayer(nn.Module):
         return delta, res
 
 
+    def step(self, positions: torch.Tensor, delta: torch.Tensor | None, residual: torch.Tensor,
+             cache: KV8Cache, new: CacheStep, first: bool, seen: tuple | None = None):
+        """One block on the residual stream of new tokens (see :meth:`Qwen2Attention.step`); returns
+        the pending delta, as :meth:`forward` does."""
+        self.build_panels(positions.shape[0])
+        try:
+            x = self.input_layernorm.residual_norm(residual, delta)
+            delta = self.self_attn.step(positions, x, residual, cache, new, first, seen)
+            x = self.post_attention_layernorm.residual_norm(residual, delta)
+            return self.mlp.step_residual(x, residual)
+        finally:
+            self.clear_panels()
+
+
 class Qwen2DecoderLayer(DecoderLayer):
 
     def __init__(self, mes_config: MESConfig) -> None:
@@ -313,6 +358,20 @@ class DecoderModel(nn.Module):
                 hidden_states, residual = layer(positions, hidden_states, residual)
             delta, res = self.layers[-1].forward_last_rows(positions, hidden_states, residual, rows)
             return self.norm.residual_norm(res, delta)
+
+    def step(self, input_ids: torch.Tensor, positions: torch.Tensor, rows: torch.Tensor, caches,
+             new: CacheStep, first: bool, seen: tuple | None = None) -> torch.Tensor:
+        """Final hidden states ``[B, H]`` of the rows ``rows`` (int64 ``[B]``) of new tokens whose
+        predecessors ``caches`` (one :class:`KV8Cache` a layer) hold; the new tokens are stored
+        there.  ``first``: all of them begin their sequences.  Not split over micro-batches."""
+        with batch_schedule(positions) if first else contextlib.nullcontext():
+            residual = self.embed_tokens.forward_f32(input_ids)
+            delta = None
+            for layer, cache in zip(self.layers, caches, strict=True):
+                delta = layer.step(positions, delta, residual, cache, new, first, seen)
+        if delta is not None:
+            delta = delta.index_select(0, rows)
+        return self.norm.residual_norm(residual.index_select(0, rows), delta)
 
     def _overlap_split(self, positions: torch.Tensor) -> int | None:
         """Token index of the sequence start nearest the middle of the batch, or None when
