@@ -62,6 +62,43 @@ __device__ __forceinline__ uint2 quantise8(const float (&f)[8], const Divisor& b
   return make_uint2(o[0], o[1]);
 }
 
+// Eight codes of scale `was` -> codes of by.scale, as quantise8 gives them for fl(code * was).  A code
+// times the ratio, a little less and a little more than it, encloses the quotient, and rounding is
+// monotone: where both give one code, that is it.  (Ties are rare here, the ratio being arbitrary.)
+template <int kKind>
+__device__ __forceinline__ uint2 requantise8(uint2 c, float was, const Divisor& by) {
+  float f[8];
+  kv8::decode4<kKind>(c.x, f);
+  kv8::decode4<kKind>(c.y, f + 4);
+  const float ratio = was * by.inv, lo = ratio * (1.f - 4.76837158e-7f), hi = ratio * (1.f + 4.76837158e-7f);
+  uint32_t o[2], differ = by.direct || !(was >= 8.6736174e-19f);
+  if (kKind == kv8::kInt8) {
+    uint32_t t[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      t[e] = __float_as_uint(fmaf(f[e], lo, 12582912.f));
+      differ |= t[e] ^ __float_as_uint(fmaf(f[e], hi, 12582912.f));
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      o[i] = __byte_perm(__byte_perm(t[4 * i], t[4 * i + 1], 0x0040), __byte_perm(t[4 * i + 2], t[4 * i + 3], 0x0040), 0x5410);
+  } else {
+    auto pack = [&](int i, float r) {
+      return __nv_cvt_float2_to_fp8x2(make_float2(f[4 * i] * r, f[4 * i + 1] * r), __NV_SATFINITE, __NV_E4M3) |
+             (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(f[4 * i + 2] * r, f[4 * i + 3] * r), __NV_SATFINITE, __NV_E4M3) << 16;
+    };
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      o[i] = pack(i, lo);
+      differ |= o[i] ^ pack(i, hi);
+    }
+  }
+  if (differ == 0) return make_uint2(o[0], o[1]);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) f[e] *= was;
+  return quantise8<kKind>(f, by);
+}
+
 // Rows of one run handled by a warp, and the block shape that follows: a run of P tokens takes
 // P / kRows warps, and a block holds at least four warps, so small pages share a block.
 constexpr int kRows = 16;
@@ -170,13 +207,7 @@ kv8_append_kernel(const __nv_bfloat16* __restrict__ Kn, int64_t ldk, const __nv_
   if (old > 0 && now > was) {
     for (int slot = slot0; slot < min(old, slot0 + kRows); slot += 2) {
       uint2* at = reinterpret_cast<uint2*>(dst + (slot - slot0) * kv8::kD);
-      const uint2 c = *at;
-      float f[8];
-      kv8::decode4<kKind>(c.x, f);
-      kv8::decode4<kKind>(c.y, f + 4);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) f[e] *= was;
-      *at = quantise8<kKind>(f, by);
+      *at = requantise8<kKind>(*at, was, by);
     }
   }
   if (sums && side == 0 && col == 0)
@@ -186,9 +217,9 @@ kv8_append_kernel(const __nv_bfloat16* __restrict__ Kn, int64_t ldk, const __nv_
 }
 
 // ------------------------------------------ read ---------------------------------------
-// out[i] = code * scale of pages[i], rounded to bf16: four 16-byte loads and eight 16-byte stores a
-// thread, a block for a piece of a page.
-constexpr int kReadChunks = 4;
+// out[i] = code * scale of pages[i], rounded to bf16: a lane turns 8 codes into one 16-byte store, so
+// that a warp's stores cover whole lines; a block does a piece of a page, a thread eight times.
+constexpr int kReadChunks = 8;
 template <int kKind>
 __global__ void __launch_bounds__(256)
 kv8_read_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ scales,
@@ -198,34 +229,25 @@ kv8_read_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ sca
   const bool ok = page >= 0 && page < num_pages;
   if (!ok && threadIdx.x == 0) record(MES_ERR_INVALID);
   const int first = blockIdx.y * kReadChunks * 256 + threadIdx.x;
-  uint4 v[kReadChunks];
+  const uint2* src = reinterpret_cast<const uint2*>(codes) + (ok ? page * page_chunks : 0) + first;
+  const float* sc = scales + (ok ? page * (page_chunks >> run_shift) : 0);
+  uint4* dst = out + n * page_chunks + first;
+  uint2 v[kReadChunks];
   float s[kReadChunks];
 #pragma unroll
   for (int i = 0; i < kReadChunks; ++i) {
-    const int r = first + 256 * i;
-    v[i] = make_uint4(0, 0, 0, 0);
-    s[i] = 0.f;
-    if (ok && r < page_chunks) {
-      v[i] = __ldg(reinterpret_cast<const uint4*>(codes) + page * page_chunks + r);
-      s[i] = __ldg(scales + page * (page_chunks >> run_shift) + (r >> run_shift));
-    }
+    const bool in = ok && first + 256 * i < page_chunks;
+    v[i] = in ? __ldg(src + 256 * i) : make_uint2(0, 0);
+    s[i] = in ? __ldg(sc + ((first + 256 * i) >> run_shift)) : 0.f;
   }
 #pragma unroll
   for (int i = 0; i < kReadChunks; ++i) {
-    const int r = first + 256 * i;
-    if (r >= page_chunks) return;
-    const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-    uint32_t u[8];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      float f[4];
-      kv8::decode4<kKind>(w[e], f);
-      u[2 * e] = mes::pack_bf16x2(f[0] * s[i], f[1] * s[i]);
-      u[2 * e + 1] = mes::pack_bf16x2(f[2] * s[i], f[3] * s[i]);
-    }
-    uint4* dst = out + 2 * (n * page_chunks + r);
-    dst[0] = make_uint4(u[0], u[1], u[2], u[3]);
-    dst[1] = make_uint4(u[4], u[5], u[6], u[7]);
+    if (first + 256 * i >= page_chunks) return;
+    float f[8];
+    kv8::decode4<kKind>(v[i].x, f);
+    kv8::decode4<kKind>(v[i].y, f + 4);
+    dst[256 * i] = make_uint4(mes::pack_bf16x2(f[0] * s[i], f[1] * s[i]), mes::pack_bf16x2(f[2] * s[i], f[3] * s[i]),
+                              mes::pack_bf16x2(f[4] * s[i], f[5] * s[i]), mes::pack_bf16x2(f[6] * s[i], f[7] * s[i]));
   }
 }
 
@@ -462,17 +484,8 @@ kv8_compact_kernel(uint8_t* codes, float* scales, float* sums, const int32_t* __
   for (int i = 0; i < kRows / 4; ++i) {
     const float was = __shfl_sync(0xffffffffu, s, 4 * i + (lane >> 3));
     if (was != now) {
-      const uint32_t w[4] = {v[i].x, v[i].y, v[i].z, v[i].w};
-      uint2 o[2];
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        float f[8];
-        kv8::decode4<kKind>(w[2 * e], f);
-        kv8::decode4<kKind>(w[2 * e + 1], f + 4);
-#pragma unroll
-        for (int q = 0; q < 8; ++q) f[q] *= was;
-        o[e] = quantise8<kKind>(f, by);
-      }
+      const uint2 o[2] = {requantise8<kKind>(make_uint2(v[i].x, v[i].y), was, by),
+                          requantise8<kKind>(make_uint2(v[i].z, v[i].w), was, by)};
       v[i] = make_uint4(o[0].x, o[0].y, o[1].x, o[1].y);
     }
     if (ok)
@@ -544,7 +557,7 @@ extern "C" int mes_kv8_read(int dtype, const void* codes, const float* scales, c
   if (!codes || !scales || !pages || !out) return MES_ERR_INVALID;
   if (!kv8::aligned(codes, 16) || !kv8::aligned(out, 16) || !kv8::aligned(scales, 4) || !kv8::aligned(pages, 4))
     return MES_ERR_ALIGN;
-  const int run_shift = __builtin_ctz((unsigned)page_size * D / 16);
+  const int run_shift = __builtin_ctz((unsigned)page_size * D / 8);
   const int page_chunks = (2 * Hkv) << run_shift;
   if (n > 0x7fffffffll || n > 0x7fffffffffffffffll / ((int64_t)page_chunks * 32)) return MES_ERR_INVALID;
   const dim3 grid((unsigned)n, (unsigned)((page_chunks + 256 * kReadChunks - 1) / (256 * kReadChunks)));
