@@ -147,8 +147,8 @@ __device__ __forceinline__ void convert(uint32_t w, uint32_t& a, uint32_t& b) {
 __device__ __forceinline__ int units_of(const Params& p, int len) {
   return p.whole > 0 ? p.whole : len > 0 ? (len + kUnit - 1) / kUnit : 1;
 }
-template <int N>
-__device__ __forceinline__ int row_tiles(int n, int G) { return (n * G + 8 * N - 1) / (8 * N); }
+template <int kRows>
+__device__ __forceinline__ int row_tiles(int n, int G) { return (n * G + kRows - 1) / kRows; }
 
 struct Seq {
   int r0, n, len;
@@ -168,6 +168,278 @@ __device__ __forceinline__ Seq sequence(const Params& p, int b) {
 
 // First unit of block i's share.
 __device__ __forceinline__ int share(int64_t units, int i, int blocks) { return (int)(units * i / blocks); }
+
+// A block's share of the line of units, with row tiles of kRows query rows.
+struct Found {
+  int b, base;          // sequence of a unit and the units before it
+  Seq s;
+};
+struct Segment {        // the units of one item that a block has
+  int h, row_base, rows, item0, units, stop;
+  Seq s;
+};
+struct Tile {           // 32 keys: the cache rows of its halves, how many of them exist, and their scales
+  int row[2], halves;
+  float2 ks, vs;
+};
+
+template <int kRows>
+struct Line {
+  const Params& p;
+  int* prefix;          // units before every `coarse`-th sequence, and all
+  int coarse, marks, first, end;
+
+  // The whole block; returns false where it has no share.
+  __device__ bool set_up(int* warp_sum) {
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    coarse = (p.B + kMaxPrefix - 1) / kMaxPrefix;
+    marks = (p.B + coarse - 1) / coarse;
+    int total = 0;
+    for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+      const int b = b0 + tid;
+      int x = 0;
+      if (b < p.B) {
+        const Seq s = sequence(p, b);
+        x = s.n > 0 ? units_of(p, s.len) * p.Hkv * row_tiles<kRows>(s.n, p.G) : 0;
+      }
+      const int mine = x;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      __syncthreads();
+      if (lane == 31) warp_sum[warp] = x;
+      __syncthreads();
+      int before = total;
+      for (int w = 0; w < warp; ++w) before += warp_sum[w];
+      if (b < p.B && b % coarse == 0) prefix[b / coarse] = before + x - mine;
+      for (int w = 0; w < kWarps; ++w) total += warp_sum[w];
+    }
+    if (tid == 0) prefix[marks] = total;
+    __syncthreads();
+    const int grain = p.whole > 0 ? p.whole : 1;     // a multiple of this many units for each block
+    const int blocks = min((int)gridDim.x, total / grain);
+    if ((int)blockIdx.x >= blocks) return false;
+    first = share(total / grain, blockIdx.x, blocks) * grain;
+    end = share(total / grain, blockIdx.x + 1, blocks) * grain;
+    return true;
+  }
+  __device__ __forceinline__ Found find(int u) const {
+    int lo = 0, hi = marks;     // prefix[lo] <= u < prefix[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (prefix[mid] <= u) lo = mid; else hi = mid;
+    }
+    Found f = {lo * coarse, prefix[lo], sequence(p, lo * coarse)};
+    // Past sequences that end before u (those without query rows have no units).
+    while (true) {
+      const int mine = f.s.n > 0 ? units_of(p, f.s.len) * p.Hkv * row_tiles<kRows>(f.s.n, p.G) : 0;
+      if (f.base + mine > u || f.b + 1 >= p.B) return f;
+      f.base += mine;
+      f.s = sequence(p, ++f.b);
+    }
+  }
+  __device__ __forceinline__ Segment segment(int u) const {
+    Segment g;
+    const Found at = find(u);
+    g.s = at.s;
+    g.units = units_of(p, g.s.len);
+    const int tiles = row_tiles<kRows>(g.s.n, p.G), rest = u - at.base, item = rest / g.units;
+    g.h = item / tiles;
+    g.row_base = (item - g.h * tiles) * kRows;
+    g.rows = min(kRows, g.s.n * p.G - g.row_base);
+    g.item0 = u - (rest - item * g.units);
+    g.stop = min(end, g.item0 + g.units);
+    return g;
+  }
+  // Tile `sub` of unit u.
+  __device__ __forceinline__ Tile tile(int u, int sub) const {
+    Tile t = {{0, 0}, 0, make_float2(0.f, 0.f), make_float2(1.f, 1.f)};
+    if (u >= end) return t;
+    const Found at = find(u);
+    const Seq s = at.s;
+    const int units = units_of(p, s.len), rest = u - at.base, item = rest / units;
+    const int t0 = (rest - item * units) * kUnit + sub * kTile;
+    const int h = item / row_tiles<kRows>(s.n, p.G);
+    int64_t page[2] = {0, 0};
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+      if (t0 + 16 * half < s.len) {
+        page[half] = p.table[(int64_t)at.b * p.width + ((t0 + 16 * half) >> p.page_shift)];
+        ++t.halves;
+      }
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      if (page[half] < 0 || page[half] >= p.num_pages) {
+        atomicCAS(&g_err_kv8_attention, 0, MES_ERR_INVALID);
+        page[half] = 0;
+      }
+      page[half] = page[half] * 2 * p.Hkv + h;       // the run of K; that of V is Hkv further
+      t.row[half] = (int)(page[half] * p.P + ((t0 + 16 * half) & (p.P - 1)));
+    }
+    if (t.halves > 0) {
+      t.ks.x = p.scales[page[0]];
+      t.vs.x = p.scales[page[0] + p.Hkv];
+    }
+    if (t.halves > 1) {
+      t.ks.y = p.scales[page[1]];
+      t.vs.y = p.scales[page[1] + p.Hkv];
+    }
+    return t;
+  }
+  // Sixteen values of a query row of a segment: task e is part e % 8 of row e / 8.
+  __device__ __forceinline__ const __nv_bfloat16* q_source(const Segment& g, int e) const {
+    const int q = g.row_base + (e >> 3), i = q / p.G;
+    return p.q + (int64_t)(g.s.r0 + i) * p.ldq + (g.h * p.G + q - i * p.G) * kv8::kD + (e & 7) * 16;
+  }
+};
+
+// One lane: a tile's copies into a stage.
+__device__ __forceinline__ void load_tile(const Params& p, const CUtensorMap& map, const Tile& t, uint8_t* k, uint64_t* bar) {
+  const int vrow = p.Hkv << p.page_shift;
+  if (p.P >= kTile) {       // one box of 32 rows a side
+    mes::mbar_arrive_expect_tx(bar, kStageBytes);
+    mes::tma_load_2d(k, &map, bar, 0, t.row[0]);
+    mes::tma_load_2d(k + kHalfBytes, &map, bar, 0, t.row[0] + vrow);
+  } else {                  // pages of 16: a box for each half that holds tokens
+    mes::mbar_arrive_expect_tx(bar, t.halves * (kStageBytes / 2));
+    mes::tma_load_2d(k, &map, bar, 0, t.row[0]);
+    mes::tma_load_2d(k + kHalfBytes, &map, bar, 0, t.row[0] + vrow);
+    if (t.halves == 2) {
+      mes::tma_load_2d(k + kHalfBytes / 2, &map, bar, 0, t.row[1]);
+      mes::tma_load_2d(k + kHalfBytes + kHalfBytes / 2, &map, bar, 0, t.row[1] + vrow);
+    }
+  }
+}
+// A tile's factors: K scale, log2 and reciprocal of the V scale.  V codes of scale 0 count as 0, so
+// their factor is free, here 1; the mark is a reciprocal of -1.
+__device__ __forceinline__ void tile_factors(const Tile& t, float2& lv, float2& iv) {
+  lv = make_float2(t.vs.x == 0.f ? 0.f : log2f(t.vs.x), t.vs.y == 0.f ? 0.f : log2f(t.vs.y));
+  iv = make_float2(t.vs.x == 0.f ? -1.f : 1.f / t.vs.x, t.vs.y == 0.f ? -1.f : 1.f / t.vs.y);
+}
+// Part `part` of a query row: f16 times a power of two that brings the row's largest value near
+// 2^8, as the B fragments of its four steps; returns the logit factor of the row.  The eight lanes
+// of a row call it together.
+template <int kKind>
+__device__ __forceinline__ float q_fragments(const uint4 (&v)[2], bool real, float scale, uint2 (&frag)[4]) {
+  const __nv_bfloat162* hv = reinterpret_cast<const __nv_bfloat162*>(v);
+  float f[16], amax = 0.f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float2 t = real ? __bfloat1622float2(hv[j]) : make_float2(0.f, 0.f);
+    f[2 * j] = t.x;
+    f[2 * j + 1] = t.y;
+    amax = fmaxf(amax, fmaxf(fabsf(t.x), fabsf(t.y)));
+  }
+#pragma unroll
+  for (int o = 4; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+  // 2^e just below the row's maximum, within what both powers of two can be.
+  const int ex = min(max((int)((__float_as_uint(amax) >> 23) & 255) - 127, -110), 120);
+  const float down = __uint_as_float((uint32_t)(127 + 8 - ex) << 23), up = __uint_as_float((uint32_t)(127 - 8 + ex) << 23);
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const float e0 = f[4 * w] * down, e1 = f[4 * w + 1] * down, e2 = f[4 * w + 2] * down, e3 = f[4 * w + 3] * down;
+    const __half2 lo2 = kKind == kv8::kInt8 ? __floats2half2_rn(e0, e2) : __floats2half2_rn(e0, e1);
+    const __half2 hi2 = kKind == kv8::kInt8 ? __floats2half2_rn(e1, e3) : __floats2half2_rn(e2, e3);
+    frag[w] = make_uint2(*reinterpret_cast<const uint32_t*>(&lo2), *reinterpret_cast<const uint32_t*>(&hi2));
+  }
+  return scale * 1.4426950408889634f * up;
+}
+
+// From the logits of a tile to the B fragments of P: S holds products of query rows and codes on
+// entry, logits (in the exp2 domain) after.  Value e of S[t][mt] is key t0 + 16 mt + 8 (e / 2) +
+// key_of(g), row 8 t + 2 c + e % 2.  p' = exp2(s + log2(vs) - m): m is a reference that need not be
+// the maximum, only near it: it moves when a value passes 2^kMost, where f16 would end, so most
+// tiles neither reduce over lanes nor touch O.
+template <int N, bool kSums>
+__device__ __forceinline__ void weights(const Params& p, float (&S)[N][2][4], float (&O)[N][8][4], float (&m)[N][2],
+                                        float (&l)[N][2], uint2 (&P)[N][2], const float (&qs)[N][2], const int (&last)[N][2],
+                                        const int64_t (&logit_row)[N][2], float2 ks, float2 lv, float2 iv, int t0, int len,
+                                        bool masked, int kg) {
+  float x[N][2][4], mx = -INFINITY;
+#pragma unroll
+  for (int t = 0; t < N; ++t)
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        S[t][mt][e] *= (mt == 0 ? ks.x : ks.y) * qs[t][e & 1];
+        x[t][mt][e] = S[t][mt][e] + ((mt == 0 ? lv.x : lv.y) - m[t][e & 1]);
+      }
+  if (kSums) {
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int key = t0 + 16 * mt + 8 * (e >> 1) + kg;
+          if (logit_row[t][e & 1] >= 0 && key < len)
+            p.logits[logit_row[t][e & 1] + key] = key > last[t][e & 1] ? -INFINITY : S[t][mt][e];
+        }
+  }
+  if (masked) {
+    __syncwarp();       // keeps this a branch: as selects it would cost every tile
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+      for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (t0 + 16 * mt + 8 * (e >> 1) + kg > last[t][e & 1]) x[t][mt][e] = -INFINITY;
+  }
+#pragma unroll
+  for (int t = 0; t < N; ++t)
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt)
+      mx = fmaxf(mx, fmaxf(fmaxf(x[t][mt][0], x[t][mt][1]), fmaxf(x[t][mt][2], x[t][mt][3])));
+  if (__any_sync(0xffffffffu, mx > kMost)) {
+#pragma unroll
+    for (int t = 0; t < N; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        // The row's largest value of this tile, without the old reference.
+        float top = -INFINITY;
+#pragma unroll
+        for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+          for (int i2 = e; i2 < 4; i2 += 2)
+            if (x[t][mt][i2] != -INFINITY) top = fmaxf(top, S[t][mt][i2] + (mt == 0 ? lv.x : lv.y));
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        const float now = fmaxf(m[t][e], top - kShift);
+        if (now > m[t][e]) {
+          const float alpha = ex2(m[t][e] - now);
+          l[t][e] *= alpha;
+#pragma unroll
+          for (int d = 0; d < 8; ++d) {
+            O[t][d][e] *= alpha;
+            O[t][d][2 + e] *= alpha;
+          }
+          m[t][e] = now;
+#pragma unroll
+          for (int mt = 0; mt < 2; ++mt)
+#pragma unroll
+            for (int i2 = e; i2 < 4; i2 += 2)
+              if (x[t][mt][i2] != -INFINITY) x[t][mt][i2] = S[t][mt][i2] + ((mt == 0 ? lv.x : lv.y) - now);
+        }
+      }
+  }
+#pragma unroll
+  for (int t = 0; t < N; ++t)
+#pragma unroll
+    for (int mt = 0; mt < 2; ++mt) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x[t][mt][e] = ex2(x[t][mt][e]);
+      const float inv = fabsf(mt == 0 ? iv.x : iv.y);
+      l[t][0] = fmaf(x[t][mt][0] + x[t][mt][2], inv, l[t][0]);
+      l[t][1] = fmaf(x[t][mt][1] + x[t][mt][3], inv, l[t][1]);
+      const __half2 p0 = __floats2half2_rn(x[t][mt][0], x[t][mt][1]), p1 = __floats2half2_rn(x[t][mt][2], x[t][mt][3]);
+      P[t][mt] = make_uint2(transpose8(*reinterpret_cast<const uint32_t*>(&p0)),
+                            transpose8(*reinterpret_cast<const uint32_t*>(&p1)));
+    }
+}
 
 template <int kKind, int N, bool kSums>
 __global__ void __launch_bounds__(kThreads, blocks_per_sm(N))
@@ -190,157 +462,24 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
   }
   // The join may be launched as soon as every block of this grid runs (it waits for their end).
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-  // Units before each sequence, or, of many, every `coarse`-th.
-  const int coarse = (p.B + kMaxPrefix - 1) / kMaxPrefix;
-  int total = 0;
-  for (int b0 = 0; b0 < p.B; b0 += kThreads) {
-    const int b = b0 + tid;
-    int x = 0;
-    if (b < p.B) {
-      const Seq s = sequence(p, b);
-      x = s.n > 0 ? units_of(p, s.len) * p.Hkv * row_tiles<N>(s.n, p.G) : 0;
-    }
-    const int mine = x;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    __syncthreads();
-    if (lane == 31) sh.warp_sum[warp] = x;
-    __syncthreads();
-    int before = total;
-    for (int w = 0; w < warp; ++w) before += sh.warp_sum[w];
-    if (b < p.B && b % coarse == 0) sh.prefix[b / coarse] = before + x - mine;
-    for (int w = 0; w < kWarps; ++w) total += sh.warp_sum[w];
-  }
-  const int marks = (p.B + coarse - 1) / coarse;
-  if (tid == 0) sh.prefix[marks] = total;
-  __syncthreads();
-  const int grain = p.whole > 0 ? p.whole : 1;     // a multiple of this many units for each block
-  const int blocks = min((int)gridDim.x, total / grain);
-  if ((int)blockIdx.x >= blocks) return;
-  const int first = share(total / grain, blockIdx.x, blocks) * grain;
-  const int end = share(total / grain, blockIdx.x + 1, blocks) * grain;
+  Line<kRows> line{p, sh.prefix};
+  if (!line.set_up(sh.warp_sum)) return;
+  const int first = line.first, end = line.end;
 
-  struct Found {
-    int b, base;        // sequence of a unit and the units before it
-    Seq s;
-  };
-  auto find = [&](int u) {
-    int lo = 0, hi = marks;     // prefix[lo] <= u < prefix[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) >> 1;
-      if (sh.prefix[mid] <= u) lo = mid; else hi = mid;
-    }
-    Found f = {lo * coarse, sh.prefix[lo], sequence(p, lo * coarse)};
-    // Past sequences that end before u (those without query rows have no units).
-    while (true) {
-      const int mine = f.s.n > 0 ? units_of(p, f.s.len) * p.Hkv * row_tiles<N>(f.s.n, p.G) : 0;
-      if (f.base + mine > u || f.b + 1 >= p.B) return f;
-      f.base += mine;
-      f.s = sequence(p, ++f.b);
-    }
-  };
-
-  // ---- the warp's tiles: unit first + i is its tile i ----
-  // Lane j holds what tiles 32 i + j need: the cache rows of its halves and its scales.
-  int t_row0 = 0, t_row1 = 0, t_halves = 0;
-  float2 t_ks = make_float2(0.f, 0.f), t_vs = make_float2(1.f, 1.f), t_lv = t_ks, t_iv = t_ks;
-  auto look_up = [&](int i0) {
-    const int u = first + i0 + lane;
-    t_halves = 0;
-    t_ks = make_float2(0.f, 0.f);
-    t_vs = make_float2(1.f, 1.f);
-    if (u >= end) return;
-    const Found at = find(u);
-    const int b = at.b;
-    const Seq s = at.s;
-    const int units = units_of(p, s.len), rest = u - at.base, item = rest / units;
-    const int t0 = (rest - item * units) * kUnit + warp * kTile;
-    const int h = item / row_tiles<N>(s.n, p.G);
-    int64_t page[2] = {0, 0};
-#pragma unroll
-    for (int half = 0; half < 2; ++half)
-      if (t0 + 16 * half < s.len) {
-        page[half] = p.table[(int64_t)b * p.width + ((t0 + 16 * half) >> p.page_shift)];
-        ++t_halves;
-      }
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      if (page[half] < 0 || page[half] >= p.num_pages) {
-        atomicCAS(&g_err_kv8_attention, 0, MES_ERR_INVALID);
-        page[half] = 0;
-      }
-      page[half] = page[half] * 2 * p.Hkv + h;       // the run of K; that of V is Hkv further
-    }
-    t_row0 = (int)(page[0] * p.P + (t0 & (p.P - 1)));
-    t_row1 = (int)(page[1] * p.P + ((t0 + 16) & (p.P - 1)));
-    if (t_halves > 0) {
-      t_ks.x = p.scales[page[0]];
-      t_vs.x = p.scales[page[0] + p.Hkv];
-    }
-    if (t_halves > 1) {
-      t_ks.y = p.scales[page[1]];
-      t_vs.y = p.scales[page[1] + p.Hkv];
-    }
-  };
-  auto load = [&](int i) {       // one lane: tile i's copies into stage i % kStages
-    uint64_t* bar = &sh.full[warp][i % kStages];
-    uint8_t* k = sh.ring[warp][i % kStages];
-    const int vrow = p.Hkv << p.page_shift;
-    if (p.P >= kTile) {       // one box of 32 rows a side
-      mes::mbar_arrive_expect_tx(bar, kStageBytes);
-      mes::tma_load_2d(k, &map, bar, 0, t_row0);
-      mes::tma_load_2d(k + kHalfBytes, &map, bar, 0, t_row0 + vrow);
-    } else {                  // pages of 16: a box for each half that holds tokens
-      mes::mbar_arrive_expect_tx(bar, t_halves * (kStageBytes / 2));
-      mes::tma_load_2d(k, &map, bar, 0, t_row0);
-      mes::tma_load_2d(k + kHalfBytes, &map, bar, 0, t_row0 + vrow);
-      if (t_halves == 2) {
-        mes::tma_load_2d(k + kHalfBytes / 2, &map, bar, 0, t_row1);
-        mes::tma_load_2d(k + kHalfBytes + kHalfBytes / 2, &map, bar, 0, t_row1 + vrow);
-      }
-    }
-  };
-  auto issue = [&](int i) {      // the whole warp: tile i
+  // The warp's tiles: tile `warp` of unit first + i is its i-th.  Lane j holds tile 32 i + j.
+  Tile t_tile;
+  float2 t_lv, t_iv;
+  auto issue = [&](int i) {      // the whole warp: tile i into stage i % kStages
     if (first + i >= end) return;
     const bool mine = lane == (i & 31);
-    if ((i & 31) == 0) look_up(i);
-    if (mine && t_halves > 0) load(i);
-    if ((i & 31) == 0) {         // the scales arrive behind the first copy
-      // V codes of scale 0 count as 0, so their factor is free, here 1; the mark is a reciprocal of -1.
-      t_lv = make_float2(t_vs.x == 0.f ? 0.f : log2f(t_vs.x), t_vs.y == 0.f ? 0.f : log2f(t_vs.y));
-      t_iv = make_float2(t_vs.x == 0.f ? -1.f : 1.f / t_vs.x, t_vs.y == 0.f ? -1.f : 1.f / t_vs.y);
-    }
+    if ((i & 31) == 0) t_tile = line.tile(first + i + lane, warp);
+    if (mine && t_tile.halves > 0) load_tile(p, map, t_tile, sh.ring[warp][i % kStages], &sh.full[warp][i % kStages]);
+    if ((i & 31) == 0) tile_factors(t_tile, t_lv, t_iv);      // the scales arrive behind the first copy
     if (mine) {
-      sh.sc[warp][i % kStages][0] = t_ks;
+      sh.sc[warp][i % kStages][0] = t_tile.ks;
       sh.sc[warp][i % kStages][1] = t_lv;
       sh.sc[warp][i % kStages][2] = t_iv;
     }
-  };
-  // ---- segments: the units of one item that this block has ----
-  struct Segment {
-    int h, row_base, rows, item0, units, stop;
-    Seq s;
-  };
-  auto segment = [&](int u) {
-    Segment g;
-    const Found at = find(u);
-    g.s = at.s;
-    g.units = units_of(p, g.s.len);
-    const int tiles = row_tiles<N>(g.s.n, p.G), rest = u - at.base, item = rest / g.units;
-    g.h = item / tiles;
-    g.row_base = (item - g.h * tiles) * kRows;
-    g.rows = min(kRows, g.s.n * p.G - g.row_base);
-    g.item0 = u - (rest - item * g.units);
-    g.stop = min(end, g.item0 + g.units);
-    return g;
-  };
-  // A thread has sixteen values of a query row (of N / 2 rows for N == 4).
-  auto q_source = [&](const Segment& g, int e) {
-    const int q = g.row_base + (e >> 3), i = q / p.G;
-    return p.q + (int64_t)(g.s.r0 + i) * p.ldq + (g.h * p.G + q - i * p.G) * kv8::kD + (e & 7) * 16;
   };
   // Copies the rows of a segment in, while the one before is worked on (32 rows have no room).
   auto q_ahead = [&](const Segment& g) {
@@ -348,13 +487,13 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
     for (int e = tid; e < kRows * 8; e += kThreads)
       if ((e >> 3) < g.rows) {
         uint4* dst = (N == 1 ? sh.raw1[e >> 3] : sh.raw[e >> 3]) + 2 * (e & 7);
-        const __nv_bfloat16* src = q_source(g, e);
+        const __nv_bfloat16* src = line.q_source(g, e);
         copy16_async(dst, src);
         copy16_async(dst + 1, src + 8);
       }
   };
   for (int i = 0; i < kStages; ++i) issue(i);
-  Segment seg = segment(first);
+  Segment seg = line.segment(first);
   q_ahead(seg);
 
   uint32_t phase = 0;           // bit s: parity of stage s's next load
@@ -365,55 +504,28 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
     const int unit0 = u - item0, start = s.len - s.n;
     if (N <= 2) asm volatile("cp.async.wait_all;" ::: "memory");
     __syncthreads();            // the previous segment's readers of q / o are done
-    // Query rows: f16 times a power of two that brings the row's largest value near 2^8.
     for (int e = tid; e < kRows * 8; e += kThreads) {
       const int r = e >> 3, part = e & 7;
-      float f[16];
-      float amax = 0.f;
+      uint4 v[2] = {};
       if (r < rows) {
-        uint4 v[2];
-        if (N <= 2) {
-          const uint4* src = (N == 1 ? sh.raw1[r] : sh.raw[r]) + 2 * part;
-          v[0] = src[0];
-          v[1] = src[1];
-        } else {
-          const uint4* src = reinterpret_cast<const uint4*>(q_source(seg, e));
-          v[0] = __ldg(src);
-          v[1] = __ldg(src + 1);
-        }
-        const __nv_bfloat162* hv = reinterpret_cast<const __nv_bfloat162*>(v);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          const float2 t = __bfloat1622float2(hv[j]);
-          f[2 * j] = t.x;
-          f[2 * j + 1] = t.y;
-          amax = fmaxf(amax, fmaxf(fabsf(t.x), fabsf(t.y)));
-        }
-        if (part == 0) sh.last[r] = start + (row_base + r) / p.G;
-      } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j) f[j] = 0.f;
-        if (part == 0) sh.last[r] = 0x7fffffff;
+        const uint4* src = N == 1 ? sh.raw1[r] + 2 * part : N == 2 ? sh.raw[r] + 2 * part
+                                                                   : reinterpret_cast<const uint4*>(line.q_source(seg, e));
+        v[0] = src[0];
+        v[1] = src[1];
+      }
+      uint2 frag[4];
+      const float qs = q_fragments<kKind>(v, r < rows, p.scale, frag);
+      if (part == 0) {
+        sh.qscale[r] = qs;
+        sh.last[r] = r < rows ? start + (row_base + r) / p.G : 0x7fffffff;
       }
 #pragma unroll
-      for (int o = 4; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
-      // 2^e just below the row's maximum, within what both powers of two can be.
-      const int ex = min(max((int)((__float_as_uint(amax) >> 23) & 255) - 127, -110), 120);
-      const float down = __uint_as_float((uint32_t)(127 + 8 - ex) << 23), up = __uint_as_float((uint32_t)(127 - 8 + ex) << 23);
-      if (part == 0) sh.qscale[r] = p.scale * 1.4426950408889634f * up;
-      const int cc = part & 3, u0 = (part >> 2) * 4, fl = (r & 7) * 4 + cc;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float e0 = f[4 * w] * down, e1 = f[4 * w + 1] * down, e2 = f[4 * w + 2] * down, e3 = f[4 * w + 3] * down;
-        const __half2 lo2 = kKind == kv8::kInt8 ? __floats2half2_rn(e0, e2) : __floats2half2_rn(e0, e1);
-        const __half2 hi2 = kKind == kv8::kInt8 ? __floats2half2_rn(e1, e3) : __floats2half2_rn(e2, e3);
-        uint2* frag = N == 1 ? &sh.q1[u0 + w][fl] : &sh.q[r >> 3][u0 + w][fl];
-        *frag = make_uint2(*reinterpret_cast<const uint32_t*>(&lo2), *reinterpret_cast<const uint32_t*>(&hi2));
-      }
+      for (int w = 0; w < 4; ++w)
+        (N == 1 ? sh.q1 : sh.q[r >> 3])[(part >> 2) * 4 + w][(r & 7) * 4 + (part & 3)] = frag[w];
     }
     __syncthreads();
     if (stop < end) {
-      seg = segment(stop);
+      seg = line.segment(stop);
       q_ahead(seg);
     }
     // This lane's rows are 8 t + 2 c + e of tile t.
@@ -507,94 +619,8 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
             }
           }
         }
-        // ---- weights: p' = exp2(s + log2(vs) - m) ----
-        // m is a reference that need not be the maximum, only near it: it moves when a value
-        // passes 2^kMost, where f16 would end, so most tiles neither reduce over lanes nor touch O.
-        const bool masked = t0 + kTile - 1 > first_last;
-        // Value e of x[t][mt]: key 16 mt + 8 (e / 2) + key_of(g), row 8 t + 2 c + e % 2.
-        float x[N][2][4], mx = -INFINITY;
-#pragma unroll
-        for (int t = 0; t < N; ++t)
-#pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              S[t][mt][e] *= (mt == 0 ? ks.x : ks.y) * qs[t][e & 1];
-              x[t][mt][e] = S[t][mt][e] + ((mt == 0 ? lv.x : lv.y) - m[t][e & 1]);
-            }
-        if (kSums) {
-#pragma unroll
-          for (int t = 0; t < N; ++t)
-#pragma unroll
-            for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e) {
-                const int key = t0 + 16 * mt + 8 * (e >> 1) + kg;
-                if (logit_row[t][e & 1] >= 0 && key < s.len)
-                  p.logits[logit_row[t][e & 1] + key] = key > last[t][e & 1] ? -INFINITY : S[t][mt][e];
-              }
-        }
-        if (masked) {
-          __syncwarp();       // keeps this a branch: as selects it would cost every tile
-#pragma unroll
-          for (int t = 0; t < N; ++t)
-#pragma unroll
-            for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-              for (int e = 0; e < 4; ++e)
-                if (t0 + 16 * mt + 8 * (e >> 1) + kg > last[t][e & 1]) x[t][mt][e] = -INFINITY;
-        }
-#pragma unroll
-        for (int t = 0; t < N; ++t)
-#pragma unroll
-          for (int mt = 0; mt < 2; ++mt)
-            mx = fmaxf(mx, fmaxf(fmaxf(x[t][mt][0], x[t][mt][1]), fmaxf(x[t][mt][2], x[t][mt][3])));
-        if (__any_sync(0xffffffffu, mx > kMost)) {
-#pragma unroll
-          for (int t = 0; t < N; ++t)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              // The row's largest value of this tile, without the old reference.
-              float top = -INFINITY;
-#pragma unroll
-              for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-                for (int i2 = e; i2 < 4; i2 += 2)
-                  if (x[t][mt][i2] != -INFINITY) top = fmaxf(top, S[t][mt][i2] + (mt == 0 ? lv.x : lv.y));
-#pragma unroll
-              for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-              const float now = fmaxf(m[t][e], top - kShift);
-              if (now > m[t][e]) {
-                const float alpha = ex2(m[t][e] - now);
-                l[t][e] *= alpha;
-#pragma unroll
-                for (int d = 0; d < 8; ++d) {
-                  O[t][d][e] *= alpha;
-                  O[t][d][2 + e] *= alpha;
-                }
-                m[t][e] = now;
-#pragma unroll
-                for (int mt = 0; mt < 2; ++mt)
-#pragma unroll
-                  for (int i2 = e; i2 < 4; i2 += 2)
-                    if (x[t][mt][i2] != -INFINITY) x[t][mt][i2] = S[t][mt][i2] + ((mt == 0 ? lv.x : lv.y) - now);
-              }
-            }
-        }
         uint2 P[N][2];      // B fragments of the two 16-key steps
-#pragma unroll
-        for (int t = 0; t < N; ++t)
-#pragma unroll
-          for (int mt = 0; mt < 2; ++mt) {
-#pragma unroll
-            for (int e = 0; e < 4; ++e) x[t][mt][e] = ex2(x[t][mt][e]);
-            const float inv = fabsf(mt == 0 ? iv.x : iv.y);
-            l[t][0] = fmaf(x[t][mt][0] + x[t][mt][2], inv, l[t][0]);
-            l[t][1] = fmaf(x[t][mt][1] + x[t][mt][3], inv, l[t][1]);
-            const __half2 p0 = __floats2half2_rn(x[t][mt][0], x[t][mt][1]), p1 = __floats2half2_rn(x[t][mt][2], x[t][mt][3]);
-            P[t][mt] = make_uint2(transpose8(*reinterpret_cast<const uint32_t*>(&p0)),
-                                  transpose8(*reinterpret_cast<const uint32_t*>(&p1)));
-          }
+        weights<N, kSums>(p, S, O, m, l, P, qs, last, logit_row, ks, lv, iv, t0, s.len, t0 + kTile - 1 > first_last, kg);
         // ---- O^T += V^T P^T: tile d of O is values 16 g + 2 d and one more of the head ----
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
@@ -752,8 +778,11 @@ kv8_join_kernel(const Params p, int grid) {
   __shared__ float2 part_ml[kWarps];
   if (kSums) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  // Every block waits for the attention kernel's end before it ends itself, whether it has work or
+  // not: what follows this kernel may rely on that one.
+  auto wait = [] { asm volatile("griddepcontrol.wait;" ::: "memory"); };
   const int64_t at = blockIdx.x * (int64_t)(kWarps / W) + warp / W;
-  if (at >= (int64_t)p.T * p.Hq) return;
+  if (at >= (int64_t)p.T * p.Hq) return wait();
   const int token = (int)(at / p.Hq), head = (int)(at - (int64_t)token * p.Hq), h = head / p.G;
   // The token's sequence and the units before it and in all, from the lengths alone: this part
   // runs while the attention kernel does.
@@ -762,7 +791,7 @@ kv8_join_kernel(const Params p, int grid) {
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     Seq x = {0, 0, 0};
     if (b0 + lane < p.B) x = sequence(p, b0 + lane);
-    const int mine = x.n > 0 ? units_of(p, x.len) * p.Hkv * row_tiles<N>(x.n, p.G) : 0;
+    const int mine = x.n > 0 ? units_of(p, x.len) * p.Hkv * row_tiles<kRows>(x.n, p.G) : 0;
     total += __reduce_add_sync(0xffffffffu, mine);
     before += __reduce_add_sync(0xffffffffu, x.r0 + x.n <= token ? mine : 0);
     const uint32_t found = __ballot_sync(0xffffffffu, x.n > 0 && token >= x.r0 && token < x.r0 + x.n);
@@ -773,16 +802,16 @@ kv8_join_kernel(const Params p, int grid) {
       s.len = __shfl_sync(0xffffffffu, x.len, src);
     }
   }
-  if (s.n <= 0) return;
+  if (s.n <= 0) return wait();
   const int blocks = min(grid, total);
   const int row = (token - s.r0) * p.G + head - h * p.G, tile = row / kRows;
   const int units = units_of(p, s.len);
-  const int u0 = before + (h * row_tiles<N>(s.n, p.G) + tile) * units, u1 = u0 + units;
+  const int u0 = before + (h * row_tiles<kRows>(s.n, p.G) + tile) * units, u1 = u0 + units;
   // The blocks whose shares meet [u0, u1).
   int from = (int)((int64_t)u0 * blocks / total);
   while (from + 1 < blocks && share(total, from + 1, blocks) <= u0) ++from;
   while (from > 0 && share(total, from, blocks) > u0) --from;
-  if (share(total, from + 1, blocks) >= u1) return;         // not cut
+  if (share(total, from + 1, blocks) >= u1) return wait();         // not cut
   const int to = [&] {                                     // one past the last of them
     int i = (int)((int64_t)(u1 - 1) * blocks / total);
     while (i + 1 < blocks && share(total, i + 1, blocks) < u1) ++i;
@@ -792,7 +821,7 @@ kv8_join_kernel(const Params p, int grid) {
   const int local = row - tile * kRows;
   // Only the item's first block can have it as its second segment.
   auto slot = [&](int i) { return ((int64_t)2 * i + (i == from && share(total, i, blocks) < u0 ? 1 : 0)) * kRows + local; };
-  asm volatile("griddepcontrol.wait;" ::: "memory");       // the partial results are there
+  wait();                                                  // the partial results are there
   // Each of the W warps takes every W-th partial result; its loads do not wait for one another.
   float mx = -INFINITY, sum = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);

@@ -280,7 +280,7 @@ __device__ __forceinline__ uint2 ld_dsmem_u32x2(uint32_t addr) {
   asm volatile("ld.shared::cluster.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(addr) : "memory");
   return v;
 }
-__global__ void __launch_bounds__(kSelThreads)
+__global__ void __launch_bounds__(kSelThreads, 1)
 kv8_select_kernel(const float* __restrict__ sums, const int32_t* __restrict__ table, int64_t width,
                   const int32_t* __restrict__ ctx, int Hkv, int page_shift, int64_t num_pages, int keep,
                   int recent, int cap, int ranks, bool vectors, int32_t* __restrict__ kept,
