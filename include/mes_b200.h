@@ -283,8 +283,8 @@ int mes_awq_gemm_on_panel(int epilogue, const void* X, int64_t ldx, const void* 
 /* Y = X * W for 1 to 16 rows: the projections of a token step.  `epilogue` as for
  * mes_awq_gemm_ws: 0 Y bf16 [M, N] = X W (+ bias), 1 Y f32 [M, N] += X W (+ bias), 2 Y bf16
  * [M, N/2] = silu(gate) * up with gate and up columns interleaved in blocks of 16 (bias NULL).
- * W = (q - z) * s is used exactly (mes_awq_gemm rounds it to bf16 first); fp32 accumulation in
- * a fixed order.  X: bf16 [M, K], pitch ldx elements; qweight_mes, qzeros, scales, bias as for
+ * W = (q - z) * s is used exactly (mes_awq_gemm rounds it to bf16 first) for |X| < 2^67; larger
+ * values overflow to infinity or NaN.  fp32 accumulation in a fixed order.  X: bf16 [M, K], pitch ldx elements; qweight_mes, qzeros, scales, bias as for
  * mes_awq_gemm.  group_size 32, 64 or 128; K % 128 == 0; N % 8 == 0 (N % 32 == 0 for
  * epilogue 2); ldx % 8 == 0.  X and qweight_mes 16-byte aligned, scales 8, qzeros 4, Y to its
  * elements.  M = 0 does nothing; M > 16 is MES_ERR_INVALID. */
@@ -304,7 +304,8 @@ int mes_awq_gemv(int epilogue, const void* X, int64_t ldx, const int32_t* qweigh
  * D == 128; P = page_size is 16, 32, 64 or 128; num_pages * 2 * Hkv * P < 2^31 rows.
  * max_new: an upper bound on the new tokens of one sequence, known to the host.  Lengths and
  * pages are read on the device; ones that lie outside T, the table or the cache are skipped and
- * record MES_ERR_INVALID as device error.  Sequences must not share pages that are written. */
+ * record MES_ERR_INVALID as device error.  Sequences must not share pages that a call writes:
+ * those of new tokens, and, where a call has sums, every page. */
 
 /* Quantises new keys and values into the cache.  K, V: bf16 rows of pitch ldk / ldv elements,
  * Hkv heads of D.  The scale of a (page, side, head) becomes max(old, amax|new| / Q), Q = 127

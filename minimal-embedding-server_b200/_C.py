@@ -721,7 +721,8 @@ def kv8_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
                                  P, pages, scale, out.data_ptr(), ws.data_ptr(), size, _stream(codes))
     if st:
         _check(st, "mes_kv8_attention")
-    launch_count += 2 if sums is None else 3
+    # A short table's items are dealt whole: no second kernel joins them.
+    launch_count += (1 if width * P <= 512 else 2) + (sums is not None)
     return out
 
 

@@ -61,10 +61,16 @@ class IncrementalEmbedder:
     def _pages_for(self, tokens: int) -> int:
         return -(-tokens // self.page_size)
 
-    def _take(self, n: int) -> list[int]:
+    def _need(self, n: int) -> None:
         if n > len(self._free):
             raise _C.MesError(f"the cache has {len(self._free)} free pages of {self.page_size} tokens, {n} are needed")
+
+    def _take(self, n: int) -> list[int]:
+        self._need(n)
         return [self._free.pop() for _ in range(n)]
+
+    def _over(self, tokens: int) -> bool:
+        return self.budget is not None and tokens > self.budget + self.budget // 4
 
     def _int32(self, values) -> torch.Tensor:
         return torch.as_tensor(np.asarray(values, dtype=np.int32)).to(self.device, non_blocking=True)
@@ -142,6 +148,8 @@ class IncrementalEmbedder:
             return torch.empty(0, self.model.norm.hidden_size, dtype=torch.float32, device=self.device)
         counts = [len(t) for t in tokens]
         need = [self._pages_for(t.cached + n) - len(t.pages) for t, n in zip(texts, counts)]
+        # Those that eviction copies to are there before anything runs, so that a text is extended whole or not at all.
+        self._need(sum(need) + sum(self._pages_for(self.budget) for t, n in zip(texts, counts) if self._over(t.cached + n)))
         pages = self._take(sum(need))
         for t, n in zip(texts, need):
             t.pages += [pages.pop() for _ in range(n)]
@@ -163,8 +171,7 @@ class IncrementalEmbedder:
             t.cached += n
             t.position += n
         out = _C.last_token_l2(hidden, torch.arange(len(texts), device=self.device))
-        if self.budget is not None:
-            self._evict([t for t in texts if t.cached > self.budget + self.budget // 4])
+        self._evict([t for t in texts if self._over(t.cached)])
         return out
 
     def _evict(self, texts) -> None:

@@ -113,6 +113,21 @@ def test_a_budget_keeps_the_cache_small(qwen3):
     assert sorted(emb._free) == list(range(60))
 
 
+def test_no_room_for_an_eviction_changes_nothing(qwen3):
+    worker, _ = qwen3
+    rng = np.random.default_rng(11)
+    emb = IncrementalEmbedder(worker.model, num_pages=8, page_size=16, budget=64)
+    (h,), _ = emb.add([_ids(rng, 80)])            # 5 pages, and no eviction yet
+    with pytest.raises(_C.MesError, match="free pages"):
+        emb.extend([h], [_ids(rng, 1)])           # 1 more, and 4 to copy to
+    assert emb.cached_tokens(h) == 80 and len(emb._free) == 3
+    with pytest.raises(_C.MesError, match="free pages"):
+        emb.add([_ids(rng, 81)])
+    assert len(emb._free) == 3
+    emb.drop([h])
+    assert sorted(emb._free) == list(range(8))
+
+
 def test_a_window_keeps_the_last_tokens(qwen3):
     """With as many recent tokens as the budget, what is kept is the end of the unlimited cache,
     re-rounded at most once a page."""
