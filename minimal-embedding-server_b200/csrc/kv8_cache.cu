@@ -287,6 +287,8 @@ kv8_select_kernel(const float* __restrict__ sums, const int32_t* __restrict__ ta
                   int32_t* __restrict__ new_lens) {
   extern __shared__ __align__(16) uint32_t cached[];
   __shared__ SelShared sh;
+  // The compaction may be launched as soon as every block of this grid runs (it waits for their end).
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = ranks > 1 ? static_cast<int>(mes::cluster_ctarank()) : 0;
   const int item = blockIdx.x / ranks, b = item / Hkv, h = item - b * Hkv;
@@ -453,6 +455,7 @@ kv8_compact_kernel(uint8_t* codes, float* scales, float* sums, const int32_t* __
       record(MES_ERR_INVALID);
     }
   }
+  asm volatile("griddepcontrol.wait;" ::: "memory");      // the kept tokens are there; every block waits
   // Lane l looks up token l of the warp's rows (the upper lanes once more).
   const int slot0 = warp % Run::kRunWarps * kRows;
   const int place = j * P + slot0 + (lane & (kRows - 1));
@@ -619,9 +622,17 @@ extern "C" int mes_kv8_evict(int dtype, void* codes, float* scales, float* sums,
     using Run = Shape<P>;
     const dim3 grid((unsigned)(B * new_width), run_blocks(Hkv, Run::kRuns));
     auto kernel = dtype == kv8::kInt8 ? kv8_compact_kernel<kv8::kInt8, P> : kv8_compact_kernel<kv8::kE4m3, P>;
-    kernel<<<grid, Run::kThreads, 0, (cudaStream_t)stream>>>(
-        (uint8_t*)codes, scales, sums, block_table, table_width, new_table, (int)new_width, kept, (int)keep,
-        Hkv, num_pages);
-    return mes_host::from_cuda(cudaGetLastError());
+    cudaLaunchAttribute early = {};
+    early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    early.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t next = {};
+    next.gridDim = grid;
+    next.blockDim = dim3(Run::kThreads);
+    next.stream = (cudaStream_t)stream;
+    next.attrs = &early;
+    next.numAttrs = 1;
+    return mes_host::from_cuda(cudaLaunchKernelEx(
+        &next, kernel, (uint8_t*)codes, scales, sums, block_table, table_width, new_table, (int)new_width,
+        (const int32_t*)kept, (int)keep, Hkv, num_pages));
   });
 }
