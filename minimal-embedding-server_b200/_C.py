@@ -612,7 +612,9 @@ def _kv8_cache(codes: torch.Tensor, scales: torch.Tensor, sums: torch.Tensor | N
     dev = codes.get_device()
     if not (dev >= 0 and two == 2 and D == 128 and P in KV8_PAGE_SIZES and codes.is_contiguous()
             and scales.dtype is _F32 and scales.shape == (pages, 2, Hkv) and scales.get_device() == dev
-            and scales.is_contiguous() and sums is None):
+            and scales.is_contiguous()
+            and (sums is None or (sums.dtype is _F32 and sums.shape == (pages, Hkv, P) and sums.get_device() == dev
+                                  and sums.is_contiguous()))):
         _need(two == 2 and P in KV8_PAGE_SIZES and D == 128 and codes.is_contiguous(),
               "codes must be contiguous [pages, 2, Hkv, P, 128] with P one of 16, 32, 64, 128")
         _arg(scales, "scales", codes, torch.float32, (pages, 2, Hkv), contiguous=True)

@@ -177,8 +177,9 @@ struct Segment {        // the units of one item that a block has
   int h, row_base, rows, item0, units, stop;
   Seq s;
 };
-struct Tile {           // 32 keys: the cache rows of its halves, how many of them exist, and their scales
-  int row[2], halves;
+struct Tile {           // 32 keys: the pages and the rows of its halves (of the page, then of the cache), how
+  int page[2], row[2];  // many of them exist, the kv head, their scales
+  int halves, h;
   float2 ks, vs;
 };
 
@@ -291,40 +292,43 @@ struct Line {
     g.stop = min(end, g.item0 + g.units);
     return g;
   }
-  // Tile `sub` of unit u.
+  // Tile `sub` of unit u, in two steps with a load each: its pages, then their scales.
   __device__ __forceinline__ Tile tile(int u, int sub) const {
-    Tile t = {{0, 0}, 0, make_float2(0.f, 0.f), make_float2(1.f, 1.f)};
+    Tile t = {{0, 0}, {0, 0}, 0, 0, make_float2(0.f, 0.f), make_float2(1.f, 1.f)};
     if (u >= end) return t;
     const Found at = find(u);
     const Seq s = at.s;
     const int units = units_of(p, s.len), rest = u - at.base, item = rest / units;
     const int t0 = (rest - item * units) * kUnit + sub * kTile;
-    const int h = item / row_tiles<kRows>(s.n, p.G);
-    int64_t page[2] = {0, 0};
+    t.h = item / row_tiles<kRows>(s.n, p.G);
 #pragma unroll
     for (int half = 0; half < 2; ++half)
       if (t0 + 16 * half < s.len) {
-        page[half] = p.table[(int64_t)at.b * p.width + ((t0 + 16 * half) >> p.page_shift)];
+        t.page[half] = p.table[(int64_t)at.b * p.width + ((t0 + 16 * half) >> p.page_shift)];
+        t.row[half] = (t0 + 16 * half) & (p.P - 1);
         ++t.halves;
       }
+    return t;
+  }
+  __device__ __forceinline__ void resolve(Tile& t) const {
+    int64_t run[2];
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-      if (page[half] < 0 || page[half] >= p.num_pages) {
+      if (t.page[half] < 0 || t.page[half] >= p.num_pages) {
         atomicCAS(&g_err_kv8_attention, 0, MES_ERR_INVALID);
-        page[half] = 0;
+        t.page[half] = 0;
       }
-      page[half] = page[half] * 2 * p.Hkv + h;       // the run of K; that of V is Hkv further
-      t.row[half] = (int)(page[half] * p.P + ((t0 + 16 * half) & (p.P - 1)));
+      run[half] = (int64_t)t.page[half] * 2 * p.Hkv + t.h;       // that of K; that of V is Hkv further
+      t.row[half] += (int)(run[half] * p.P);
     }
     if (t.halves > 0) {
-      t.ks.x = p.scales[page[0]];
-      t.vs.x = p.scales[page[0] + p.Hkv];
+      t.ks.x = p.scales[run[0]];
+      t.vs.x = p.scales[run[0] + p.Hkv];
     }
     if (t.halves > 1) {
-      t.ks.y = p.scales[page[1]];
-      t.vs.y = p.scales[page[1] + p.Hkv];
+      t.ks.y = p.scales[run[1]];
+      t.vs.y = p.scales[run[1] + p.Hkv];
     }
-    return t;
   }
   // Sixteen values of a query row of a segment: task e is part e % 8 of row e / 8.
   __device__ __forceinline__ const __nv_bfloat16* q_source(const Segment& g, int e) const {
@@ -509,7 +513,10 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
   float2 t_lv, t_iv;
   auto copy = [&](int i) {       // the whole warp: tile i into stage i % kStages
     if (first + i >= end) return;
-    if ((i & 31) == 0) t_tile = line.tile(first + i + lane, warp);
+    if ((i & 31) == 0) {
+      if (i > 0) t_tile = line.tile(first + i + lane, warp);
+      line.resolve(t_tile);
+    }
     if (lane == (i & 31) && t_tile.halves > 0)
       load_tile(p, map, t_tile, sh.ring[warp][i % kStages], &sh.full[warp][i % kStages]);
   };
@@ -532,10 +539,14 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
         copy16_async(dst + 1, src + 8);
       }
   };
-  for (int i = 0; i < kStages; ++i) copy(i);
+  // What is loaded arrives while the next is worked out: pages, query rows, tiles, scales.
+  t_tile = line.tile(first + lane, warp);
   Segment seg = line.segment(first);
   q_ahead(seg);
-  for (int i = 0; i < kStages; ++i) factors(i);
+  for (int i = 0; i < kStages; ++i) copy(i);
+  // The factors come last; 32 rows have no registers to hold the scales until then (2 of 37 us).
+  if (N > 2)
+    for (int i = 0; i < kStages; ++i) factors(i);
 
   uint32_t phase = 0;           // bit s: parity of stage s's next load
   bool ok = true;
@@ -562,6 +573,8 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
       for (int w = 0; w < 4; ++w)
         sh.q[r >> 3][(part >> 2) * 4 + w][(r & 7) * 4 + (part & 3)] = frag[w];
     }
+    if (N <= 2 && u == first)
+      for (int i = 0; i < kStages; ++i) factors(i);
     __syncthreads();
     if (stop < end) {
       seg = line.segment(stop);
