@@ -21,6 +21,10 @@
 // code at bits 0-3 or 4-7 of a half is the bf16 number q 2^-133 or q 2^-129 (bf16 is linear from
 // zero up to 2^-125), so one shift and four masks make eight operands.  X is multiplied by 2^60 or
 // 2^56 to meet them, which is exact for |x| < 2^67, and the result by 2^73.
+//
+// Measured: 8 rows of 4096 x 24576 with silu 16.2 us (52 MB, 3.2 TB/s, half of the copy rate: the
+// integer pipe that masks the codes is 45% busy, and 384 blocks share 148 SMs unevenly); 1 row of
+// 2048 x 1024 3.6 us, a launch and one round of loads.
 #include "common.cuh"
 
 namespace {
@@ -343,7 +347,7 @@ extern "C" int mes_awq_gemv(int epilogue, const void* X, int64_t ldx, const int3
                              CU_TENSOR_MAP_SWIZZLE_128B))
     return MES_ERR_CUDA;
   // Two tiles of features share the work on X where that leaves two blocks an SM (8 rows of
-  // 4096 x 24576: 16.4 us against 19.6 with one).
+  // 4096 x 24576: 16.2 us against 19.6 with one).
   const bool wide = N >= 4 * (int64_t)mes_host::sm_count() * kFeatures;
   return launch_any(group_size, wide, M > 8, epilogue, map_w, map_x, qzeros, scales, bias, Y, ldy, M, N, K, stream);
 }
