@@ -8,10 +8,12 @@
 //
 // Work: a (sequence, kv head, row tile) is an item, 128 keys of it a unit.  The units of all items
 // form one line that is cut evenly among the blocks, whatever the lengths are, so no block waits
-// for a long sequence; beginning an item counts as a few units.  An item cut between blocks leaves at most two partial results a block (its
-// first and its last segment), joined by a second kernel.  The lengths stay on the device.  Where
-// no sequence can be long (the table has room for four units at most), items are dealt whole and
-// there is no second kernel: 500 tokens and one query take 7.9 us with the join.
+// for a long sequence; beginning an item counts as a few units.  An item cut between blocks leaves
+// at most two partial results a block (its first and its last segment), joined by a second kernel.
+// The lengths stay on the device.  Where no sequence can be long (the table has room for four units
+// at most), items are dealt whole and there is no second kernel: 256 sequences of 100 to 500 tokens
+// take 51 instead of 71 us.  One of 500 alone takes 10.5 instead of 7.9, but its call, which the
+// host bounds, 14.5 instead of 17.
 //
 // A block is four warps.  Each takes 32 keys of a unit for itself: its own ring of TMA tiles
 // (128-byte swizzle, so the 16-byte reads below meet no bank conflict), its own running maximum
@@ -26,6 +28,11 @@
 // Scales: a page's K scale multiplies its logits.  Its V scale vs goes into the exponent,
 // p' = exp2(s + log2(vs) - m), with m a running reference near the maximum of s + log2(vs): p'
 // stays within f16 whatever the scales are, and the softmax sum adds p' / vs.
+//
+// Measured: two sequences of 131072 tokens, 8 kv heads, one query each 93 us (537 MB, 5.8 TB/s, 0.88 of
+// the copy rate); 64 of 100 to 8192 tokens 100 us (0.85).  With 138 query rows for each kv head the
+// tensor pipe is 41% busy (250 TFLOP/s over 16384 tokens): two warps a scheduler, which is what the
+// registers leave, do not hide one another's latencies.
 #include "kv8.cuh"
 
 namespace {
@@ -983,8 +990,8 @@ kv8_sums_kernel(const Params p, float* sums) {
     if (t + j < s.len) at[j] = old[j] + add[j];
 }
 
-// Row tiles as large as the most query rows of a kv head, at most 32: a converted key feeds one
-// product for each 8 rows.
+// Row tiles as large as the most query rows of a kv head, at most 32, which is what a thread's
+// registers hold: a converted key feeds one product for each 8 rows.
 int row_factor(int64_t max_new, int G) { return max_new * G <= 8 ? 1 : max_new * G <= 16 ? 2 : 4; }
 int max_blocks(int N) { return mes_host::sm_count() * blocks_per_sm(N); }
 

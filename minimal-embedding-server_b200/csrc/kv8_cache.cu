@@ -128,6 +128,8 @@ __device__ __forceinline__ float run_max(float v, float* red) {
 // run re-rounded when s grew, new tokens rounded once.  s_old counts only where the run already
 // held tokens.  Non-finite inputs do not set the scale: an infinity saturates, NaN becomes 0.
 // Each new value is read once and kept in registers between the maximum and the rounding.
+// Measured: 20 x 1000 tokens of 8 heads 29.5 us (123 MB, 4.2 TB/s, 0.64 of the copy rate); one token for
+// each of 32 sequences 2.9 us.
 template <int kKind, int P>
 __global__ void __launch_bounds__(Shape<P>::kThreads)
 kv8_append_kernel(const __nv_bfloat16* __restrict__ Kn, int64_t ldk, const __nv_bfloat16* __restrict__ Vn,
@@ -219,6 +221,7 @@ kv8_append_kernel(const __nv_bfloat16* __restrict__ Kn, int64_t ldk, const __nv_
 // ------------------------------------------ read ---------------------------------------
 // out[i] = code * scale of pages[i], rounded to bf16: a lane turns 8 codes into one 16-byte store, so
 // that a warp's stores cover whole lines; a block does a piece of a page, a thread eight times.
+// Measured: 20000 tokens of 8 heads 18 us (123 MB, 6.8 TB/s: part of the codes is still in L2).
 constexpr int kReadChunks = 8;
 template <int kKind>
 __global__ void __launch_bounds__(256)
@@ -258,6 +261,8 @@ kv8_read_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ sca
 // 11 and 10 bits, added over the cluster through distributed shared memory; then each warp walks
 // its part of the slice in token order, so the kept indices come out sorted and a tie goes to
 // the lower index.
+// Measured: 8 heads of 100003 tokens 26 us, 64 of 4096 12 us.  Latency bounds it: lengths, pages and sums
+// are loaded one after the other (6 us), and each pass has two barriers of the cluster (5 us).
 constexpr int kSelThreads = 1024, kBins = 2048, kSelWarps = kSelThreads / 32;
 
 // Larger float -> larger integer; -0 equals +0 and NaN is lowest.
@@ -435,6 +440,8 @@ kv8_select_kernel(const float* __restrict__ sums, const int32_t* __restrict__ ta
 // Compaction: run (sequence, new page, side, head) gathers its tokens in kept order.  The run's
 // scale is the largest of its sources' scales, so tokens from the source that has it move
 // unchanged and the others are re-rounded once.
+// Measured: 16384 tokens of 8 heads 16.5 us after the selection (67 MB, 4.1 TB/s; a chain of four loads,
+// index, page, scale and codes, for each run).
 template <int kKind, int P>
 __global__ void __launch_bounds__(Shape<P>::kThreads)
 kv8_compact_kernel(uint8_t* codes, float* scales, float* sums, const int32_t* __restrict__ table,
