@@ -546,8 +546,10 @@ def _gemv_args(x: torch.Tensor, qw: torch.Tensor, qz: torch.Tensor, sc: torch.Te
 
 def _gemv_call(epi: int, x, qw, qz, sc, bias, y, M: int, N: int, K: int, group_size: int) -> None:
     global launch_count
-    st = lib().mes_awq_gemv(epi, x.data_ptr(), x.stride()[0], qw.data_ptr(), qz.data_ptr(), sc.data_ptr(),
-                            None if bias is None else bias.data_ptr(), y.data_ptr(), y.stride()[0], M, N, K,
+    # One row's stride means nothing.
+    st = lib().mes_awq_gemv(epi, x.data_ptr(), x.stride()[0] if M > 1 else K, qw.data_ptr(), qz.data_ptr(),
+                            sc.data_ptr(), None if bias is None else bias.data_ptr(), y.data_ptr(),
+                            y.stride()[0] if M > 1 else N, M, N, K,
                             group_size, _stream(x))
     if st:
         _check(st, f"mes_awq_gemv ({_EPI_NAME[epi]} epilogue)")
@@ -640,11 +642,12 @@ def _kv8_batch(codes: torch.Tensor, block_table: torch.Tensor, context_lens: tor
     return B, width
 
 
-def _kv8_rows(t: torch.Tensor, name: str, codes: torch.Tensor, T: int, cols: int) -> None:
-    """Checks the packed rows ``t``: bf16 ``[T, cols]`` of unit inner stride."""
+def _kv8_rows(t: torch.Tensor, name: str, codes: torch.Tensor, T: int, cols: int) -> int:
+    """Checks the packed rows ``t``: bf16 ``[T, cols]`` of unit inner stride; returns their pitch."""
     if not (t.dtype is _BF16 and t.shape == (T, cols) and t.get_device() == codes.get_device() >= 0
             and t.stride()[1] == 1):
         _arg(t, name, codes, torch.bfloat16, (T, cols), unit_stride=True)
+    return t.stride()[0] if T > 1 else cols
 
 
 def kv8_append(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
@@ -658,9 +661,9 @@ def kv8_append(k: torch.Tensor, v: torch.Tensor, codes: torch.Tensor, scales: to
     kind, pages, Hkv, P = _kv8_cache(codes, scales, sums)
     B, width = _kv8_batch(codes, block_table, context_lens, cu_new)
     T = k.shape[0]
-    _kv8_rows(k, "k", codes, T, Hkv * 128)
-    _kv8_rows(v, "v", codes, T, Hkv * 128)
-    st = lib().mes_kv8_append(kind, k.data_ptr(), k.stride()[0], v.data_ptr(), v.stride()[0], codes.data_ptr(),
+    ldk = _kv8_rows(k, "k", codes, T, Hkv * 128)
+    ldv = _kv8_rows(v, "v", codes, T, Hkv * 128)
+    st = lib().mes_kv8_append(kind, k.data_ptr(), ldk, v.data_ptr(), ldv, codes.data_ptr(),
                               scales.data_ptr(), None if sums is None else sums.data_ptr(),
                               block_table.data_ptr(), width, cu_new.data_ptr(), context_lens.data_ptr(), B, T,
                               max_new, Hkv, 128, P, pages, _stream(codes))
@@ -707,7 +710,7 @@ def kv8_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     kind, pages, Hkv, P = _kv8_cache(codes, scales, sums)
     B, width = _kv8_batch(codes, block_table, context_lens, cu_new)
     T = q.shape[0]
-    _kv8_rows(q, "q", codes, T, num_heads * 128)
+    ldq = _kv8_rows(q, "q", codes, T, num_heads * 128)
     if out is None:
         out = torch.empty((T, num_heads * 128), dtype=_BF16, device=codes.device)
     else:
@@ -717,7 +720,7 @@ def kv8_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
         raise MesError(f"mes_kv8_attention: unsupported sizes: {T} tokens of {B} sequences (at most {max_new} "
                        f"of one), {num_heads} heads over {Hkv}")
     ws = torch.empty(size, dtype=torch.uint8, device=codes.device)
-    st = lib().mes_kv8_attention(kind, q.data_ptr(), q.stride()[0], codes.data_ptr(), scales.data_ptr(),
+    st = lib().mes_kv8_attention(kind, q.data_ptr(), ldq, codes.data_ptr(), scales.data_ptr(),
                                  None if sums is None else sums.data_ptr(), block_table.data_ptr(), width,
                                  cu_new.data_ptr(), context_lens.data_ptr(), B, T, max_new, num_heads, Hkv, 128,
                                  P, pages, scale, out.data_ptr(), ws.data_ptr(), size, _stream(codes))

@@ -319,6 +319,30 @@ def test_attention_work_split(kind, batch):
     _attend_and_check(Cache(kind, 32, 2, ctx).fill(), [1] * batch, 4)
 
 
+@pytest.mark.parametrize("new", [1, 5, 17])
+@pytest.mark.parametrize("sums", [False, True])
+def test_attention_many_items(new, sums):
+    """More units than blocks, so that shares count the items' beginnings; sequences without new tokens
+    among them, tiles of 8, 16 and 32 rows, the last of an item not full."""
+    rng = np.random.default_rng(new)
+    ctx = [1, 4000] + [int(n) for n in np.exp(rng.uniform(np.log(20), np.log(2500), 68))]
+    news = [min(c, int(n)) for c, n in zip(ctx, rng.integers(0, new + 1, 70))]
+    news[5] = new
+    _attend_and_check(Cache(torch.int8, 16, 3, ctx).fill(), news, 6, sums=sums, max_new=new)
+
+
+def test_one_row_may_have_any_stride():
+    cache = Cache(torch.int8, 16, 2, [40]).fill()
+    other = Cache(torch.int8, 16, 2, [40]).fill()
+    rows = torch.randn(3, 4 * D, device=DEV).to(torch.bfloat16)
+    got = []
+    for c, (q, k, v) in ((cache, [r[None] for r in rows]), (other, [r[:, None].t() for r in rows])):
+        k, v = k[:, :2 * D], v[:, :2 * D]
+        _C.kv8_append(k, v, c.codes, c.scales, c.table, _cu([1]), c.lens, max_new=1)
+        got.append((_C.kv8_attention(q, c.codes, c.scales, c.table, _cu([1]), c.lens, 4, 0.1, max_new=1), c.codes))
+    assert got[1][0].isfinite().all() and all(torch.equal(a, b) for a, b in zip(*got))
+
+
 @pytest.mark.parametrize("sums", [False, True])
 def test_attention_of_a_long_text_by_itself(sums):
     """Every token of a text in one call: the first sees itself only."""
