@@ -331,7 +331,8 @@ int mes_kv8_read(int dtype, const void* codes, const float* scales, const int32_
  * token's weight, summed over the new tokens and the query heads of its kv head, is added to its
  * sum.  At most 1024 sequences.  workspace: 256-byte aligned, of
  * mes_kv8_attention_workspace_size(T, B, Hq, Hkv, max_new, max_context) bytes, max_context =
- * table_width * P with sums and 0 without; its contents are undefined after the call. */
+ * table_width * P with sums and 0 without; its contents are undefined after the call.  NULL is
+ * taken where table_width * P <= 512 and there are no sums. */
 int64_t mes_kv8_attention_workspace_size(int64_t T, int64_t B, int Hq, int Hkv, int64_t max_new,
                                          int64_t max_context);
 int mes_kv8_attention(int dtype, const void* q, int64_t ldq, const void* codes,

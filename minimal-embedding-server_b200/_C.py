@@ -566,7 +566,7 @@ def awq_gemv(x: torch.Tensor, qweight_mes: torch.Tensor, qzeros: torch.Tensor,
                                  and bias.is_contiguous()):
         _arg(bias, "bias", x, torch.bfloat16, (N,), contiguous=True)
     if out is None:
-        out = torch.empty((M, N), dtype=_BF16, device=x.device)
+        out = x.new_empty(M, N)
     else:
         _arg(out, "out", x, torch.bfloat16, (M, N), unit_stride=True)
     _gemv_call(EPI_BF16, x, qweight_mes, qzeros, scales, bias, out, M, N, K, group_size)
@@ -594,7 +594,7 @@ def awq_gemv_silu(x: torch.Tensor, qweight_mes: torch.Tensor, qzeros: torch.Tens
     16 (see ``interleave_gate_up``); output ``[M, N/2]`` bf16."""
     M, N, K = _gemv_args(x, qweight_mes, qzeros, scales, group_size)
     if out is None:
-        out = torch.empty((M, N // 2), dtype=_BF16, device=x.device)
+        out = x.new_empty(M, N // 2)
     else:
         _arg(out, "out", x, torch.bfloat16, (M, N // 2), unit_stride=True)
     _gemv_call(EPI_SILU, x, qweight_mes, qzeros, scales, None, out, M, N, K, group_size)
@@ -682,7 +682,7 @@ def kv8_read(codes: torch.Tensor, scales: torch.Tensor, pages: torch.Tensor,
     if not (pages.dtype is _I32T and pages.get_device() == codes.get_device() >= 0 and pages.is_contiguous()):
         _arg(pages, "pages", codes, torch.int32, contiguous=True)
     if out is None:
-        out = torch.empty((n, 2, Hkv, P, 128), dtype=_BF16, device=codes.device)
+        out = torch.empty(n, 2, Hkv, P, 128, dtype=_BF16, device=codes.device)
     else:
         _arg(out, "out", codes, torch.bfloat16, (n, 2, Hkv, P, 128), contiguous=True)
     st = lib().mes_kv8_read(kind, codes.data_ptr(), scales.data_ptr(), pages.data_ptr(), n, Hkv, 128, P,
@@ -712,22 +712,24 @@ def kv8_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
     T = q.shape[0]
     ldq = _kv8_rows(q, "q", codes, T, num_heads * 128)
     if out is None:
-        out = torch.empty((T, num_heads * 128), dtype=_BF16, device=codes.device)
+        out = q.new_empty(T, num_heads * 128)
     else:
         _arg(out, "out", codes, torch.bfloat16, (T, num_heads * 128), contiguous=True)
+    # A short table's items are dealt whole: no partial results, no second kernel.
+    short = width * P <= 512
     size = _kv8_workspace(codes.get_device(), T, B, num_heads, Hkv, max_new, 0 if sums is None else width * P)
     if size < 0:
         raise MesError(f"mes_kv8_attention: unsupported sizes: {T} tokens of {B} sequences (at most {max_new} "
                        f"of one), {num_heads} heads over {Hkv}")
-    ws = torch.empty(size, dtype=torch.uint8, device=codes.device)
+    ws = None if short and sums is None else torch.empty(size, dtype=torch.uint8, device=codes.device)
     st = lib().mes_kv8_attention(kind, q.data_ptr(), ldq, codes.data_ptr(), scales.data_ptr(),
                                  None if sums is None else sums.data_ptr(), block_table.data_ptr(), width,
                                  cu_new.data_ptr(), context_lens.data_ptr(), B, T, max_new, num_heads, Hkv, 128,
-                                 P, pages, scale, out.data_ptr(), ws.data_ptr(), size, _stream(codes))
+                                 P, pages, scale, out.data_ptr(), None if ws is None else ws.data_ptr(),
+                                 0 if ws is None else size, _stream(codes))
     if st:
         _check(st, "mes_kv8_attention")
-    # A short table's items are dealt whole: no second kernel joins them.
-    launch_count += (1 if width * P <= 512 else 2) + (sums is not None)
+    launch_count += (1 if short else 2) + (sums is not None)
     return out
 
 
@@ -746,8 +748,8 @@ def kv8_evict(codes: torch.Tensor, scales: torch.Tensor, sums: torch.Tensor,
     if not (new_table.dtype is _I32T and new_table.shape == (B, new_width) and new_table.is_contiguous()
             and new_table.get_device() == codes.get_device() >= 0):
         _arg(new_table, "new_table", codes, torch.int32, (B, new_width), contiguous=True)
-    kept = torch.empty((B, Hkv, keep), dtype=_I32T, device=codes.device)
-    new_lens = torch.empty(B, dtype=_I32T, device=codes.device)
+    kept = context_lens.new_empty(B, Hkv, keep)
+    new_lens = context_lens.new_empty(B)
     st = lib().mes_kv8_evict(kind, codes.data_ptr(), scales.data_ptr(), sums.data_ptr(), block_table.data_ptr(),
                              width, context_lens.data_ptr(), B, new_table.data_ptr(), new_width, keep, recent,
                              Hkv, 128, P, pages, kept.data_ptr(), new_lens.data_ptr(), _stream(codes))

@@ -1082,14 +1082,17 @@ extern "C" int mes_kv8_attention(int dtype, const void* q, int64_t ldq, const vo
   if (!valid_sizes(T, B, Hq, Hkv, max_new, max_ctx)) return MES_ERR_INVALID;
   if (ldq < (int64_t)Hq * D || ldq % 8) return MES_ERR_INVALID;
   if (B == 0 || T == 0 || max_new == 0) return MES_OK;
-  if (!q || !codes || !scales || !block_table || !cu_new || !context_lens || !out || !workspace) return MES_ERR_INVALID;
+  if (!q || !codes || !scales || !block_table || !cu_new || !context_lens || !out) return MES_ERR_INVALID;
   if (!kv8::aligned(q, 16) || !kv8::aligned(codes, 16) || !kv8::aligned(scales, 4) || !kv8::aligned(sums, 4) ||
       !kv8::aligned(block_table, 4) || !kv8::aligned(cu_new, 4) || !kv8::aligned(context_lens, 4) ||
       !kv8::aligned(out, 16) || !kv8::aligned(workspace, 256))
     return MES_ERR_ALIGN;
   const int G = Hq / Hkv, N = row_factor(max_new, G);
   const Layout w = layout(T, Hq, N, max_ctx);
-  if (workspace_bytes < w.bytes) return MES_ERR_INVALID;
+  // Whole items without sums leave nothing to keep.
+  const int64_t most = (table_width * page_size + kUnit - 1) / kUnit;
+  const int whole = most <= kWholeUnits ? (int)most : 0;
+  if ((whole == 0 || sums) && (!workspace || workspace_bytes < w.bytes)) return MES_ERR_INVALID;
   // Places of the line are counted in 32 bits.
   const int64_t tiles = (max_new * G + 8 * N - 1) / (8 * N);
   if (((table_width * page_size + kUnit - 1) / kUnit + segment_cost(N)) * Hkv > 0x7fffffffll / (B * tiles)) return MES_ERR_INVALID;
@@ -1123,8 +1126,7 @@ extern "C" int mes_kv8_attention(int dtype, const void* q, int64_t ldq, const vo
   p.lse = sums ? (float*)(ws + w.lse) : nullptr;
   p.logits = sums ? (float*)(ws + w.logits) : nullptr;
   p.max_ctx = max_ctx;
-  const int64_t most = (table_width * page_size + kUnit - 1) / kUnit;
-  p.whole = most <= kWholeUnits ? (int)most : 0;
+  p.whole = whole;
   auto go = [&](auto n) {
     constexpr int kN = decltype(n)::value;
     if (dtype == kv8::kInt8)

@@ -551,6 +551,25 @@ def test_evict_scales_far_apart(kind):
 
 
 # ------------------------------------------------------------------------------ refusals
+def test_short_tables_need_no_workspace():
+    """Up to 512 tokens of table one kernel and no workspace; past it, and with sums, both are needed."""
+    lib, stream = _C.lib(), torch.cuda.current_stream().cuda_stream
+    for page, width, sums, want in ((16, 32, False, 0), (16, 33, False, 2), (128, 4, False, 0), (128, 5, False, 2), (16, 32, True, 2)):
+        cache = Cache(torch.int8, page, 2, [page * width]).fill()
+        q, out = torch.randn(1, 4 * D, device=DEV).to(torch.bfloat16), torch.zeros(1, 4 * D, dtype=torch.bfloat16, device=DEV)
+        cu = _cu([1])
+        st = lib.mes_kv8_attention(0, q.data_ptr(), 4 * D, cache.codes.data_ptr(), cache.scales.data_ptr(),
+                                   cache.sums.data_ptr() if sums else None, cache.table.data_ptr(), width, cu.data_ptr(),
+                                   cache.lens.data_ptr(), 1, 1, 1, 4, 2, D, page, cache.num_pages, 0.1, out.data_ptr(), None,
+                                   0, stream)
+        assert (st != 0) == (want != 0), (page, width, sums, st)
+        before = _C.launch_count
+        got = _C.kv8_attention(q, cache.codes, cache.scales, cache.table, cu, cache.lens, 4, 0.1, max_new=1,
+                               sums=cache.sums if sums else None)
+        assert _C.launch_count - before == (1 if page * width <= 512 else 2) + sums
+        assert st != 0 or torch.equal(got, out)
+
+
 def test_refusals():
     cache = Cache(torch.int8, 32, 2, [40]).fill()
     k = torch.zeros(1, 2 * D, dtype=torch.bfloat16, device=DEV)
