@@ -156,6 +156,7 @@ kv8_append_kernel(const __nv_bfloat16* __restrict__ Kn, int64_t ldk, const __nv_
                   const int32_t* __restrict__ ctx, int64_t T, int max_pages, int Hkv,
                   int64_t num_pages) {
   using Run = Shape<P>;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ float red[8];
   constexpr float kQ = kv8::code_max<kKind>();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -261,6 +262,7 @@ __global__ void __launch_bounds__(256)
 kv8_read_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ scales,
                 const int32_t* __restrict__ pages, int page_chunks, int run_shift, int64_t num_pages,
                 uint4* __restrict__ out) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
   const int64_t n = blockIdx.x, page = __ldg(pages + n);
   const bool ok = page >= 0 && page < num_pages;
   if (!ok && threadIdx.x == 0) record(MES_ERR_INVALID);
@@ -481,6 +483,7 @@ kv8_compact_kernel(uint8_t* codes, float* scales, float* sums, const int32_t* __
                    int64_t width, const int32_t* __restrict__ new_table, int new_width,
                    const int32_t* __restrict__ kept, int keep, int Hkv, int64_t num_pages) {
   using Run = Shape<P>;
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   __shared__ float red[8];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int b = blockIdx.x / new_width, j = blockIdx.x - b * new_width;
@@ -605,9 +608,17 @@ extern "C" int mes_kv8_read(int dtype, const void* codes, const float* scales, c
   if (n > 0x7fffffffll || n > 0x7fffffffffffffffll / ((int64_t)page_chunks * 32)) return MES_ERR_INVALID;
   const dim3 grid((unsigned)n, (unsigned)((page_chunks + 256 * kReadChunks - 1) / (256 * kReadChunks)));
   auto kernel = dtype == kv8::kInt8 ? kv8_read_kernel<kv8::kInt8> : kv8_read_kernel<kv8::kE4m3>;
-  kernel<<<grid, 256, 0, (cudaStream_t)stream>>>((const uint8_t*)codes, scales, pages, page_chunks, run_shift,
-                                                 num_pages, (uint4*)out);
-  return mes_host::from_cuda(cudaGetLastError());
+  cudaLaunchAttribute early = {};
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(256);
+  cfg.stream = (cudaStream_t)stream;
+  cfg.attrs = &early;
+  cfg.numAttrs = 1;
+  return mes_host::from_cuda(cudaLaunchKernelEx(&cfg, kernel, (const uint8_t*)codes, scales, pages, page_chunks, run_shift,
+                                                num_pages, (uint4*)out));
 }
 
 extern "C" int mes_kv8_evict(int dtype, void* codes, float* scales, float* sums,
