@@ -38,8 +38,8 @@ class IncrementalEmbedder:
         """``model``: a ``Qwen3ForCausalLM`` / ``Qwen2ForCausalLM`` on its device (e.g.
         ``GPUWorker.model``).  ``num_pages`` pages of ``page_size`` tokens are shared by all texts.
         ``budget``: cached tokens a text is cut down to once it has a quarter more, ``recent`` of
-        them (default: a quarter) the last ones; the last ``observe`` tokens of a new text give
-        its first attention weights."""
+        them (default: a quarter) the last ones; of a new text, or of more tokens than that added
+        to one, the last ``observe`` give the attention weights."""
         self.model = model.model
         layers = self.model.layers
         self.device = self.model.embed_tokens.weight.device
@@ -162,8 +162,9 @@ class IncrementalEmbedder:
         lens = self._int32([t.cached + n for t, n in zip(texts, counts)])
         step = CacheStep(table, self._int32([0, *ends]), lens, max(counts))
         seen = None
-        if first and self.budget is not None and self.observe > 0:
-            last = [min(n, self.observe) for n in counts]
+        observe = self.observe if first else max(self.observe, 1)
+        if self.budget is not None and observe > 0 and (first or max(counts) > observe):
+            last = [min(n, observe) for n in counts]
             seen = (torch.as_tensor(np.concatenate([np.arange(e - m, e) for e, m in zip(ends, last)])).to(self.device),
                     CacheStep(table, self._int32([0, *np.cumsum(last)]), lens, max(last)))
         hidden = self.model.step(ids, positions, rows, self.caches, step, first, seen)

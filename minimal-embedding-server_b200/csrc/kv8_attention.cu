@@ -1028,7 +1028,8 @@ int launch(const CUtensorMap& map, const Params& p, float* sums, void* stream) {
   const int grid = mes_host::persistent_ctas() * blocks_per_sm(N);
   kernel<<<grid, kThreads, sizeof(Smem<N>), (cudaStream_t)stream>>>(map, p);
   if (cudaGetLastError() != cudaSuccess) return MES_ERR_CUDA;
-  // The kernels that follow start while the one before them ends (programmatic launch).
+  // The kernels that follow start while the one before them ends (programmatic launch).  What they read
+  // ahead of that end is older than the attention kernel, which is launched in plain order.
   cudaLaunchAttribute attr = {};
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;

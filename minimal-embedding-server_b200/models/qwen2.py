@@ -110,8 +110,8 @@ class Qwen2Attention(nn.Module):
         """Attention block of new tokens whose predecessors are in ``cache``, added into the fp32
         residual stream.  The new tokens' keys and values are stored first.  ``first``: nothing
         was cached before, so the tokens attend to one another in 16 bits, as in ``forward``.
-        ``seen``: ``(rows, step)`` of tokens whose attention weights count towards eviction
-        although their output is not needed from the cache."""
+        ``seen``: ``(rows, step)`` of the tokens whose attention weights count towards eviction, where
+        that is not all of them."""
         qkv = self.qkv_proj.step(hidden_states)
         norms = (self.q_norm, self.k_norm) if self.apply_qk_norm else ()
         self.rotary_emb.forward_fused(positions, qkv, self.num_heads, self.num_kv_heads, *norms)
@@ -119,10 +119,10 @@ class Qwen2Attention(nn.Module):
         cache.append(k, v, new)
         if first:
             out = self.attn.forward_packed(qkv, positions)
-            if seen is not None:
-                cache.attend(q.index_select(0, seen[0]), seen[1], self.num_heads, self.scaling)
         else:
-            out = cache.attend(q, new, self.num_heads, self.scaling)
+            out = cache.attend(q, new, self.num_heads, self.scaling, track=seen is None)
+        if seen is not None:
+            cache.attend(q.index_select(0, seen[0]), seen[1], self.num_heads, self.scaling)
         return self.o_proj.step_residual(out, residual)
 
 

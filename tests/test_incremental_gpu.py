@@ -113,6 +113,23 @@ def test_a_budget_keeps_the_cache_small(qwen3):
     assert sorted(emb._free) == list(range(60))
 
 
+def test_the_last_tokens_of_a_run_give_the_weights(qwen3):
+    """Every observed query adds weights of sum 1 for each of its heads: after a text, a long and a short
+    addition the sums of a kv head tell how many queries were observed."""
+    worker, cfg = qwen3
+    rng = np.random.default_rng(12)
+    G = cfg.num_attention_heads // cfg.num_key_value_heads
+    emb = IncrementalEmbedder(worker.model, num_pages=20, page_size=16, budget=256, observe=4)
+    (h,), _ = emb.add([_ids(rng, 50)])
+    for more, seen in ((0, 4), (40, 8), (3, 11), (1, 12)):
+        if more:
+            emb.extend([h], [_ids(rng, more)])
+        n, pages = emb.cached_tokens(h), torch.tensor(emb._texts[h].pages, device=DEV)
+        for cache in emb.caches:
+            total = cache.sums[pages].transpose(0, 1).reshape(cache.sums.shape[1], -1)[:, :n].double().sum(1)
+            assert ((total - seen * G).abs() < 1e-3 * seen * G).all(), (more, total)
+
+
 def test_no_room_for_an_eviction_changes_nothing(qwen3):
     worker, _ = qwen3
     rng = np.random.default_rng(11)
