@@ -11,9 +11,15 @@ attention weight are dropped, for each layer and kv head by itself; the most rec
 Positions go on counting from the text's first token.
 
 Every layer has its own cache and all layers use the same pages, so one block table serves a step.
-Runs of at most 16 new tokens in all take the matrix-vector kernels; longer ones the GEMMs.
+Runs of at most 16 new tokens in all take the matrix-vector kernels, as CUDA graphs once their sizes come
+back; longer ones the GEMMs.  Calls are made on one stream at a time.
 """
 from __future__ import annotations
+
+import collections
+import dataclasses
+import os
+import warnings
 
 import numpy as np
 import torch
@@ -29,6 +35,37 @@ class _Text:
         self.pages: list[int] = []
         self.cached = 0
         self.position = 0
+
+
+class _Step:
+    """What a step reads, on the device: int64 ``[2 T + B]`` ids, positions and each text's last row, int32
+    ``[B width + 2 B + 1]`` block table, offsets and lengths."""
+
+    def __init__(self, device, B: int, T: int, width: int, max_new: int, longs, ints) -> None:
+        self.longs, self.ints = (torch.as_tensor(x).to(device) for x in (longs, ints))
+        self.ids, self.positions, self.rows = self.longs.split([T, T, B])
+        table, cu_new, lens = self.ints.split([B * width, B + 1, B])
+        self.cache_step = CacheStep(table.view(B, width), cu_new, lens, max_new)
+        self.texts = torch.arange(B, device=device)
+
+
+class _StepGraph:
+    """A captured step of ``B`` texts with ``T`` new tokens in all."""
+
+    def __init__(self, embedder: "IncrementalEmbedder", B: int, T: int, width: int, max_new: int) -> None:
+        self.step = _Step(embedder.device, B, T, width, max_new, np.zeros(2 * T + B, np.int64),
+                          np.zeros(B * width + 2 * B + 1, np.int32))
+        if embedder._pool is None:
+            embedder._pool = torch.cuda.graph_pool_handle()
+        self.graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(self.graph, pool=embedder._pool):
+            self.out = embedder._forward(self.step, False)
+
+    def replay(self, longs, ints) -> torch.Tensor:
+        self.step.longs.copy_(torch.as_tensor(longs))
+        self.step.ints.copy_(torch.as_tensor(ints))
+        self.graph.replay()
+        return self.out.clone()
 
 
 class IncrementalEmbedder:
@@ -56,6 +93,11 @@ class IncrementalEmbedder:
         self._free = list(range(num_pages - 1, -1, -1))
         self._texts: dict[int, _Text] = {}
         self._next = 0
+        self.use_cuda_graphs = os.environ.get("MES_CUDA_GRAPHS", "1") != "0"
+        self.max_graphs = 32
+        self._tp_size = layers[0].self_attn.o_proj.tp_size if len(layers) else 1
+        self._graphs: collections.OrderedDict[tuple, _StepGraph | None] = collections.OrderedDict()
+        self._pool = None
 
     # ------------------------------------------------------------------ pages
     def _pages_for(self, tokens: int) -> int:
@@ -147,33 +189,74 @@ class IncrementalEmbedder:
         if not texts:
             return torch.empty(0, self.model.norm.hidden_size, dtype=torch.float32, device=self.device)
         counts = [len(t) for t in tokens]
-        need = [self._pages_for(t.cached + n) - len(t.pages) for t, n in zip(texts, counts)]
+        need = [max(self._pages_for(t.cached + n) - len(t.pages), 0) for t, n in zip(texts, counts)]
         # Those that eviction copies to are there before anything runs, so that a text is extended whole or not at all.
         self._need(sum(need) + sum(self._pages_for(self.budget) for t, n in zip(texts, counts) if self._over(t.cached + n)))
         pages = self._take(sum(need))
         for t, n in zip(texts, need):
             t.pages += [pages.pop() for _ in range(n)]
-        ids = torch.as_tensor(np.concatenate(tokens)).to(self.device, non_blocking=True)
-        positions = torch.as_tensor(np.concatenate(
-            [np.arange(t.position, t.position + n, dtype=np.int64) for t, n in zip(texts, counts)])).to(self.device, non_blocking=True)
-        ends = np.cumsum(counts)
-        rows = torch.as_tensor(ends - 1).to(self.device, non_blocking=True)
-        table = self._table([t.pages for t in texts])
-        lens = self._int32([t.cached + n for t, n in zip(texts, counts)])
-        step = CacheStep(table, self._int32([0, *ends]), lens, max(counts))
-        seen = None
+        positions = [np.arange(t.position, t.position + n) for t, n in zip(texts, counts)]
+        lens = [t.cached + n for t, n in zip(texts, counts)]
         observe = self.observe if first else max(self.observe, 1)
-        if self.budget is not None and observe > 0 and (first or max(counts) > observe):
-            last = [min(n, observe) for n in counts]
-            seen = (torch.as_tensor(np.concatenate([np.arange(e - m, e) for e, m in zip(ends, last)])).to(self.device),
-                    CacheStep(table, self._int32([0, *np.cumsum(last)]), lens, max(last)))
-        hidden = self.model.step(ids, positions, rows, self.caches, step, first, seen)
+        seen = self.budget is not None and observe > 0 and (first or max(counts) > observe)
+        graph, width = None, max(len(t.pages) for t in texts)
+        if self.use_cuda_graphs and not first and not seen and sum(counts) <= _C.GEMV_MAX_ROWS and self._tp_size == 1:
+            width = max(8, 1 << (width - 1).bit_length())
+            graph = self._graph_for((len(texts), sum(counts), width, max(counts)))
+        longs, ints = self._pack(tokens, positions, counts, [t.pages for t in texts], width, lens)
+        if graph is not None:
+            out = graph.replay(longs, ints)
+        else:
+            step = _Step(self.device, len(texts), sum(counts), width, max(counts), longs, ints)
+            observed = None
+            if seen:
+                last = [min(n, observe) for n in counts]
+                rows = np.concatenate([np.arange(e - m, e) for e, m in zip(np.cumsum(counts), last)])
+                observed = (torch.as_tensor(rows).to(self.device), dataclasses.replace(
+                    step.cache_step, cu_new=self._int32([0, *np.cumsum(last)]), max_new=max(last)))
+            out = self._forward(step, first, observed)
         for t, n in zip(texts, counts):
             t.cached += n
             t.position += n
-        out = _C.last_token_l2(hidden, torch.arange(len(texts), device=self.device))
         self._evict([t for t in texts if self._over(t.cached)])
         return out
+
+    def _pack(self, tokens, positions, counts, pages, width: int, lens):
+        """What a step reads, as two host arrays (see :class:`_Step`)."""
+        ends = np.cumsum(counts)
+        table = np.zeros((len(pages), width), dtype=np.int32)
+        for row, p in zip(table, pages):
+            row[:len(p)] = p
+        return (np.concatenate([*tokens, *positions, ends - 1]).astype(np.int64, copy=False),
+                np.concatenate([table.reshape(-1), [0], ends, lens]).astype(np.int32, copy=False))
+
+    def _forward(self, step: "_Step", first: bool, observed: tuple | None = None) -> torch.Tensor:
+        hidden = self.model.step(step.ids, step.positions, step.rows, self.caches, step.cache_step, first, observed)
+        return _C.last_token_l2(hidden, step.texts)
+
+    # A token step is some ten launches a layer of a few microseconds each, less than the host needs for
+    # them, so a step of sizes that come back is captured the second time (the first, run eagerly,
+    # sets the kernels up; a step cannot be run twice, since it adds to the weights).
+    def _graph_for(self, key: tuple):
+        graph = self._graphs.get(key)
+        if graph is None and key not in self._graphs:
+            self._graphs[key] = None
+            while len(self._graphs) > self.max_graphs:
+                self._graphs.popitem(last=False)
+            return None
+        self._graphs.move_to_end(key)
+        if graph is None:
+            try:
+                graph = self._graphs[key] = _StepGraph(self, *key)
+            except Exception as exc:
+                warnings.warn(f"CUDA-graph capture of a token step failed ({exc!r}); steps run eagerly", RuntimeWarning,
+                              stacklevel=3)
+                self.use_cuda_graphs = False
+        return graph
+
+    def release_graphs(self) -> None:
+        """Drop every captured step."""
+        self._graphs.clear()
 
     def _evict(self, texts) -> None:
         if not texts:

@@ -130,6 +130,38 @@ def test_the_last_tokens_of_a_run_give_the_weights(qwen3):
             assert ((total - seen * G).abs() < 1e-3 * seen * G).all(), (more, total)
 
 
+@pytest.mark.parametrize("budget", [None, 40])
+def test_captured_steps_match_eager_ones(qwen3, budget):
+    """Steps whose sizes come back run as graphs, with the lengths and pages of each call, across page
+    and eviction boundaries; what differs is how the attention is cut (fp32 rounding)."""
+    worker, cfg = qwen3
+    G = cfg.num_attention_heads // cfg.num_key_value_heads
+    embs, got = [], []
+    for graphs in (True, False):
+        rng = np.random.default_rng(13)
+        emb = IncrementalEmbedder(worker.model, num_pages=60, page_size=16, budget=budget, observe=2)
+        emb.use_cuda_graphs = graphs
+        handles, _ = emb.add([_ids(rng, 20), _ids(rng, 33), _ids(rng, 1)])
+        out = []
+        for i in range(14):
+            some = handles[:2] if i % 3 == 2 else handles
+            out.append(emb.extend(some, [_ids(rng, 1 + (i + j) % 2) for j in range(len(some))]))
+        embs.append(emb)
+        got.append([o.cpu().numpy() for o in out])
+    captured = [g for g in embs[0]._graphs.values() if g is not None]
+    assert len(captured) >= 3 and not embs[1]._graphs
+    for a, b in zip(*got):
+        assert (_cos(a, b) > 0.9999).all(), _cos(a, b)
+    if budget is None:
+        return
+    for a, b in zip(embs[0].caches, embs[1].caches):     # every step's weights are counted once
+        ta, tb = ([c.sums[torch.tensor(e._texts[0].pages, device=DEV)].transpose(0, 1).reshape(c.sums.shape[1], -1)
+                   [:, :e.cached_tokens(0)].double().sum(1) for e, c in zip(embs, (a, b))])
+        assert ((ta - tb).abs() < 0.02 * tb).all()
+    embs[0].release_graphs()
+    assert not embs[0]._graphs
+
+
 def test_no_room_for_an_eviction_changes_nothing(qwen3):
     worker, _ = qwen3
     rng = np.random.default_rng(11)
