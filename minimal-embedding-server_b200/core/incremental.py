@@ -93,7 +93,7 @@ class IncrementalEmbedder:
         self._free = list(range(num_pages - 1, -1, -1))
         self._texts: dict[int, _Text] = {}
         self._next = 0
-        self.use_cuda_graphs = os.environ.get("MES_CUDA_GRAPHS", "1") != "0"
+        self.use_cuda_graphs = self.device.type == "cuda" and os.environ.get("MES_CUDA_GRAPHS", "1") != "0"
         self.max_graphs = 32
         self._tp_size = layers[0].self_attn.o_proj.tp_size if len(layers) else 1
         self._graphs: collections.OrderedDict[tuple, _StepGraph | None] = collections.OrderedDict()

@@ -73,7 +73,8 @@ def test_cache_entry_points_refuse():
         assert _append(**kw) == 2, kw
     assert _append(T=0, max_new=0) == 0 and _append(max_new=0) == 0
     for kw in (dict(T=-1), dict(max_new=9), dict(hq=3), dict(hq=0), dict(ldq=504), dict(ldq=516), dict(B=1025), dict(q=None),
-               dict(cu=None), dict(out=None), dict(ws=None), dict(size=0)):
+               dict(cu=None), dict(out=None), dict(ws=None, width=17), dict(size=0, width=17), dict(ws=None, sums=A),
+               dict(size=0, sums=A)):       # a short table without sums needs no workspace
         assert _attention(**kw) == 1, kw
     for kw in (dict(q=ODD8), dict(out=ODD8), dict(ws=A + 128), dict(cu=ODD2)):
         assert _attention(**kw) == 2, kw
