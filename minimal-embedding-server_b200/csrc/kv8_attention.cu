@@ -406,19 +406,17 @@ __device__ __forceinline__ void weights(const Params& p, float (&S)[N][2][4], fl
                                         float (&l)[N][2], uint2 (&P)[N][2], const float (&qs)[N][2], const int (&last)[N][2],
                                         const int64_t (&logit_row)[N][2], float2 ks, float2 lv, float2 iv, int t0, int len,
                                         bool masked, int kg) {
-  float x[N][2][4], mx = -INFINITY;
 #pragma unroll
-  for (int t = 0; t < N; ++t)
+  for (int t = 0; t < N; ++t) {
+    float x[2][4], mx = -INFINITY;
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         S[t][mt][e] *= (mt == 0 ? ks.x : ks.y) * qs[t][e & 1];
-        x[t][mt][e] = S[t][mt][e] + ((mt == 0 ? lv.x : lv.y) - m[t][e & 1]);
+        x[mt][e] = S[t][mt][e] + ((mt == 0 ? lv.x : lv.y) - m[t][e & 1]);
       }
-  if (kSums) {
-#pragma unroll
-    for (int t = 0; t < N; ++t)
+    if (kSums) {
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
@@ -427,25 +425,18 @@ __device__ __forceinline__ void weights(const Params& p, float (&S)[N][2][4], fl
           if (logit_row[t][e & 1] >= 0 && key < len)
             p.logits[logit_row[t][e & 1] + key] = key > last[t][e & 1] ? -INFINITY : S[t][mt][e];
         }
-  }
-  if (masked) {
-    __syncwarp();       // keeps this a branch: as selects it would cost every tile
-#pragma unroll
-    for (int t = 0; t < N; ++t)
+    }
+    if (masked) {
+      __syncwarp();       // keeps this a branch: as selects it would cost every tile
 #pragma unroll
       for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          if (t0 + 16 * mt + 8 * (e >> 1) + kg > last[t][e & 1]) x[t][mt][e] = -INFINITY;
-  }
+          if (t0 + 16 * mt + 8 * (e >> 1) + kg > last[t][e & 1]) x[mt][e] = -INFINITY;
+    }
 #pragma unroll
-  for (int t = 0; t < N; ++t)
-#pragma unroll
-    for (int mt = 0; mt < 2; ++mt)
-      mx = fmaxf(mx, fmaxf(fmaxf(x[t][mt][0], x[t][mt][1]), fmaxf(x[t][mt][2], x[t][mt][3])));
-  if (__any_sync(0xffffffffu, mx > kMost)) {
-#pragma unroll
-    for (int t = 0; t < N; ++t)
+    for (int mt = 0; mt < 2; ++mt) mx = fmaxf(mx, fmaxf(fmaxf(x[mt][0], x[mt][1]), fmaxf(x[mt][2], x[mt][3])));
+    if (__any_sync(0xffffffffu, mx > kMost)) {
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
         // The row's largest value of this tile, without the old reference.
@@ -454,7 +445,7 @@ __device__ __forceinline__ void weights(const Params& p, float (&S)[N][2][4], fl
         for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
           for (int i2 = e; i2 < 4; i2 += 2)
-            if (x[t][mt][i2] != -INFINITY) top = fmaxf(top, S[t][mt][i2] + (mt == 0 ? lv.x : lv.y));
+            if (x[mt][i2] != -INFINITY) top = fmaxf(top, S[t][mt][i2] + (mt == 0 ? lv.x : lv.y));
 #pragma unroll
         for (int o = 4; o < 32; o <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
         const float now = fmaxf(m[t][e], top - kShift);
@@ -471,23 +462,22 @@ __device__ __forceinline__ void weights(const Params& p, float (&S)[N][2][4], fl
           for (int mt = 0; mt < 2; ++mt)
 #pragma unroll
             for (int i2 = e; i2 < 4; i2 += 2)
-              if (x[t][mt][i2] != -INFINITY) x[t][mt][i2] = S[t][mt][i2] + ((mt == 0 ? lv.x : lv.y) - now);
+              if (x[mt][i2] != -INFINITY) x[mt][i2] = S[t][mt][i2] + ((mt == 0 ? lv.x : lv.y) - now);
         }
       }
-  }
-#pragma unroll
-  for (int t = 0; t < N; ++t)
+    }
 #pragma unroll
     for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) x[t][mt][e] = ex2(x[t][mt][e]);
+      for (int e = 0; e < 4; ++e) x[mt][e] = ex2(x[mt][e]);
       const float inv = fabsf(mt == 0 ? iv.x : iv.y);
-      l[t][0] = fmaf(x[t][mt][0] + x[t][mt][2], inv, l[t][0]);
-      l[t][1] = fmaf(x[t][mt][1] + x[t][mt][3], inv, l[t][1]);
-      const __half2 p0 = __floats2half2_rn(x[t][mt][0], x[t][mt][1]), p1 = __floats2half2_rn(x[t][mt][2], x[t][mt][3]);
+      l[t][0] = fmaf(x[mt][0] + x[mt][2], inv, l[t][0]);
+      l[t][1] = fmaf(x[mt][1] + x[mt][3], inv, l[t][1]);
+      const __half2 p0 = __floats2half2_rn(x[mt][0], x[mt][1]), p1 = __floats2half2_rn(x[mt][2], x[mt][3]);
       P[t][mt] = make_uint2(transpose8(*reinterpret_cast<const uint32_t*>(&p0)),
                             transpose8(*reinterpret_cast<const uint32_t*>(&p1)));
     }
+  }
 }
 
 template <int kKind, int N, bool kSums>
