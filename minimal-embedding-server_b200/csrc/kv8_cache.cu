@@ -457,6 +457,8 @@ kv8_select_kernel(const float* __restrict__ sums, const int32_t* __restrict__ ta
   if (lane < rank) others = ld_dsmem_u32x2(mes::mapa_shared(mes::smem_u32(&sh.greater), lane));
   uint32_t gt_before = __reduce_add_sync(0xffffffffu, others.x + (lane < warp ? sh.warp_sum[0][lane] : 0u));
   uint32_t eq_before = __reduce_add_sync(0xffffffffu, others.y + (lane < warp ? sh.warp_sum[1][lane] : 0u));
+  // No block leaves while another reads its counts: this warp has read them.
+  if (ranks > 1) asm volatile("barrier.cluster.arrive.aligned;" ::: "memory");
 #pragma unroll 4
   for (int i0 = w0; i0 < w1; i0 += 32) {
     const int i = i0 + lane;
@@ -469,7 +471,8 @@ kv8_select_kernel(const float* __restrict__ sums, const int32_t* __restrict__ ta
     gt_before += __popc(is_gt);
     eq_before += __popc(is_eq);
   }
-  if (ranks > 1) mes::cluster_sync();    // no block leaves while another reads its counts
+  __syncwarp();
+  if (ranks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
 
 // Compaction: run (sequence, new page, side, head) gathers its tokens in kept order.  The run's
