@@ -353,28 +353,40 @@ kv8_select_kernel(const float* __restrict__ sums, const int32_t* __restrict__ ta
   // last four reads past `count` is memory of its page and is not used.
   const int slice = ((n + ranks - 1) / ranks + 31) / 32 * 32;
   const int lo = min(rank * slice, n), count = min(lo + slice, n) - lo;
-  auto place = [&](int i) {
-    const int t = lo + i;
-    int64_t page = table[b * width + (t >> page_shift)];
+  bool bad = false;
+  auto page_of = [&](int i) { return table[b * width + ((lo + i) >> page_shift)]; };
+  auto place = [&](int i, int64_t page) {
     if (page < 0 || page >= num_pages) {
-      record(MES_ERR_INVALID);
+      bad = true;
       page = 0;
     }
-    return sums + ((page * Hkv + h) << page_shift) + (t & ((1 << page_shift) - 1));
+    return sums + ((page * Hkv + h) << page_shift) + ((lo + i) & ((1 << page_shift) - 1));
   };
   const int in_smem = min(count, cap);
-#pragma unroll 4
-  for (int i = 4 * tid; i < in_smem; i += 4 * kSelThreads) {
-    const float* at = place(i);
-    if (vectors) {
-      const float4 v = *reinterpret_cast<const float4*>(at);
-      *reinterpret_cast<uint4*>(cached + i) = make_uint4(order_key(v.x), order_key(v.y), order_key(v.z), order_key(v.w));
-    } else {
+  for (int i0 = 4 * tid; i0 < in_smem; i0 += 16 * kSelThreads) {      // four pages, then four loads in flight
+    int page[4];
+    float4 v[4];
 #pragma unroll
-      for (int e = 0; e < 4; ++e) cached[i + e] = order_key(at[e]);
+    for (int j = 0; j < 4; ++j) {
+      const int i = i0 + 4 * kSelThreads * j;
+      page[j] = i < in_smem ? page_of(i) : 0;
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = i0 + 4 * kSelThreads * j;
+      if (i >= in_smem) continue;
+      const float* at = place(i, page[j]);
+      v[j] = vectors ? *reinterpret_cast<const float4*>(at) : make_float4(at[0], at[1], at[2], at[3]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int i = i0 + 4 * kSelThreads * j;
+      if (i < in_smem)
+        *reinterpret_cast<uint4*>(cached + i) =
+            make_uint4(order_key(v[j].x), order_key(v[j].y), order_key(v[j].z), order_key(v[j].w));
     }
   }
-  auto load = [&](int i) { return order_key(*place(i)); };
+  auto load = [&](int i) { return order_key(*place(i, page_of(i))); };
   auto key = [&](int i) { return i < cap ? cached[i] : load(i); };
 
   uint32_t prefix = 0, want = k;      // the threshold's high bits; its place among the keys that share them
@@ -471,6 +483,7 @@ kv8_select_kernel(const float* __restrict__ sums, const int32_t* __restrict__ ta
     gt_before += __popc(is_gt);
     eq_before += __popc(is_eq);
   }
+  if (bad) record(MES_ERR_INVALID);
   __syncwarp();
   if (ranks > 1) asm volatile("barrier.cluster.wait.aligned;" ::: "memory");
 }
