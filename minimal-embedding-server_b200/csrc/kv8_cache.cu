@@ -296,8 +296,8 @@ kv8_read_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ sca
 // 11 and 10 bits, added over the cluster through distributed shared memory; then each warp walks
 // its part of the slice in token order, so the kept indices come out sorted and a tie goes to
 // the lower index.
-// Measured: 8 heads of 100003 tokens 26 us, 64 of 4096 12 us.  Latency bounds it: lengths, pages and sums
-// are loaded one after the other (6 us), and each pass has two barriers of the cluster (5 us).
+// Measured: 8 heads of 100003 tokens 24.5 us, 64 of 4096 11.8 us.  Latency bounds it: lengths, pages and
+// sums are loaded one after the other (5 us), and each pass has two barriers of the cluster (5 us).
 constexpr int kSelThreads = 1024, kBins = 2048, kSelWarps = kSelThreads / 32;
 
 // Larger float -> larger integer; -0 equals +0 and NaN is lowest.
@@ -491,7 +491,7 @@ kv8_select_kernel(const float* __restrict__ sums, const int32_t* __restrict__ ta
 // Compaction: run (sequence, new page, side, head) gathers its tokens in kept order.  The run's
 // scale is the largest of its sources' scales, so tokens from the source that has it move
 // unchanged and the others are re-rounded once.
-// Measured: 16384 tokens of 8 heads 16.5 us after the selection (67 MB, 4.1 TB/s; a chain of four loads,
+// Measured: 16384 tokens of 8 heads 16 us after the selection (67 MB, 4.2 TB/s; a chain of four loads,
 // index, page, scale and codes, for each run).
 template <int kKind, int P>
 __global__ void __launch_bounds__(Shape<P>::kThreads)
