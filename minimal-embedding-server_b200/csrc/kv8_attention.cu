@@ -30,8 +30,8 @@
 // stays within f16 whatever the scales are, and the softmax sum adds p' / vs.
 //
 // Measured: two sequences of 131072 tokens, 8 kv heads, one query each 93 us (537 MB, 5.8 TB/s, 0.88 of
-// the copy rate); 64 of 100 to 8192 tokens 100 us (0.85).  With 138 query rows for each kv head the
-// tensor pipe is 41% busy (250 TFLOP/s over 16384 tokens): two warps a scheduler, which is what the
+// the copy rate); 64 of 100 to 8192 tokens 100 us (0.85).  With 138 query rows for each kv head it
+// comes to 250 TFLOP/s (8 sequences of 16384 tokens): two warps a scheduler, which is what the
 // registers leave, do not hide one another's latencies.
 #include "kv8.cuh"
 
@@ -52,8 +52,8 @@ constexpr float kShift = 10.f, kMost = 15.f;
 // Blocks of an SM: registers and shared memory hold three with 8 query rows, two with more.
 constexpr int blocks_per_sm(int N) { return N == 1 ? 3 : 2; }
 // What beginning an item costs a block, in units of work.  Against 0: 64 ragged sequences of up to
-// 8192 tokens take 100 instead of 105 us, eight of 23 new tokens after 1500 to 4000, 34.6 instead of 38.3.
-constexpr int segment_cost(int N) { return N == 1 ? 2 : N == 2 ? 3 : 6; }
+// 8192 tokens take 100 instead of 105 us.
+constexpr int kSegmentCost = 2;
 
 // N: 8-row tiles of query rows.
 template <int N>
@@ -190,7 +190,7 @@ struct Tile {           // 32 keys: the pages and the rows of its halves (of the
   float2 ks, vs;
 };
 
-// The line of units; for the shares, each item has `segment_cost` units of nothing before its own.
+// The line of units; for the shares, each item has kSegmentCost units of nothing before its own.
 struct Count {
   int units, items;
   __device__ __forceinline__ int with(int c) const { return units + c * items; }
@@ -203,7 +203,7 @@ __device__ __forceinline__ Count count_of(const Params& p, const Seq& s) {
 // Units of nothing before an item's own: none where items are dealt whole or each unit has a block.
 template <int kRows>
 __device__ __forceinline__ int cost_of(const Params& p, int units, int grid) {
-  return p.whole > 0 || units <= grid ? 0 : segment_cost(kRows / 8);
+  return p.whole > 0 || units <= grid ? 0 : kSegmentCost;
 }
 
 template <int kRows>
@@ -541,9 +541,6 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
   Segment seg = line.segment(first);
   q_ahead(seg);
   for (int i = 0; i < kStages; ++i) copy(i);
-  // The factors come last; 32 rows have no registers to hold the scales until then (2 of 37 us).
-  if (N > 2)
-    for (int i = 0; i < kStages; ++i) factors(i);
 
   uint32_t phase = 0;           // bit s: parity of stage s's next load
   bool ok = true;
@@ -570,7 +567,7 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
       for (int w = 0; w < 4; ++w)
         sh.q[r >> 3][(part >> 2) * 4 + w][(r & 7) * 4 + (part & 3)] = frag[w];
     }
-    if (N <= 2 && u == first)
+    if (u == first)         // the first tiles' scales have arrived by now
       for (int i = 0; i < kStages; ++i) factors(i);
     __syncthreads();
     if (stop < end) {
@@ -767,7 +764,7 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
     __syncthreads();
     take_rows(warp ^ 1);
     // This warp's tile and the place of its 4 N values in a lane's 16.
-    const int tile = N == 1 ? 0 : warp * N / 4, at16 = N == 1 ? 4 * warp : N == 2 ? 8 * (warp & 1) : 0;
+    const int tile = N == 1 ? 0 : warp >> 1, at16 = N == 1 ? 4 * warp : 8 * (warp & 1);
     float fm[2] = {0.f, 0.f}, ft[2] = {0.f, 0.f}, row_m[2] = {0.f, 0.f}, row_l[2] = {0.f, 0.f};
 #pragma unroll
     for (int t = 0; t < N; ++t)
@@ -980,9 +977,10 @@ kv8_sums_kernel(const Params p, float* sums) {
     if (t + j < s.len) at[j] = old[j] + add[j];
 }
 
-// Row tiles as large as the most query rows of a kv head, at most 32, which is what a thread's
-// registers hold: a converted key feeds one product for each 8 rows.
-int row_factor(int64_t max_new, int G) { return max_new * G <= 8 ? 1 : max_new * G <= 16 ? 2 : 4; }
+// Row tiles of 8 or 16 rows: 16 sequences of 8192 tokens and 8 rows take 33.2 us in tiles of 8 and 34.6 in
+// tiles of 16.  Tiles of 32 share a converted key among more products, but their registers spill and leave
+// less room for loads in flight: 30 rows after 2048 tokens 17.5 instead of 14.5 us, 138 rows 34.1 instead of 29.8.
+int row_factor(int64_t max_new, int G) { return max_new * G <= 8 ? 1 : 2; }
 int max_blocks(int N) { return mes_host::sm_count() * blocks_per_sm(N); }
 
 constexpr int64_t up256(int64_t x) { return (x + 255) / 256 * 256; }
@@ -1027,11 +1025,10 @@ int launch(const CUtensorMap& map, const Params& p, float* sums, void* stream) {
   cfg.stream = (cudaStream_t)stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  // Few items leave many partial results each: four warps then share a row's, as long as the blocks
-  // are few too (four, instead of one: 100000 tokens and a query, 45 instead of 52 us; 80 query rows in
-  // 32 items of 2048 tokens, 25.7 instead of 23.1).
+  // Few items leave many partial results each: four warps then share a row's (100000 tokens and a query, 43.4
+  // instead of 50.4 us).  More items than that leave one block of the join little to do.
   const int64_t items = (int64_t)p.Hkv * max(p.B, (p.T * p.G + 8 * N - 1) / (8 * N));
-  const bool wide = items * 8 <= grid && (int64_t)p.T * p.Hq <= 2 * (int64_t)grid;
+  const bool wide = items * 8 <= grid;
   const int per_block = wide ? 1 : kWarps;
   cfg.gridDim = dim3((unsigned)(((int64_t)p.T * p.Hq + per_block - 1) / per_block));
   cfg.blockDim = dim3(kThreads);
@@ -1086,7 +1083,7 @@ extern "C" int mes_kv8_attention(int dtype, const void* q, int64_t ldq, const vo
   if ((whole == 0 || sums) && (!workspace || workspace_bytes < w.bytes)) return MES_ERR_INVALID;
   // Places of the line are counted in 32 bits.
   const int64_t tiles = (max_new * G + 8 * N - 1) / (8 * N);
-  if (((table_width * page_size + kUnit - 1) / kUnit + segment_cost(N)) * Hkv > 0x7fffffffll / (B * tiles)) return MES_ERR_INVALID;
+  if (((table_width * page_size + kUnit - 1) / kUnit + kSegmentCost) * Hkv > 0x7fffffffll / (B * tiles)) return MES_ERR_INVALID;
   if (sums && B * Hkv > 65535) return MES_ERR_INVALID;
   CUtensorMap map;
   const int box = page_size < kTile ? page_size : kTile;
@@ -1124,6 +1121,5 @@ extern "C" int mes_kv8_attention(int dtype, const void* q, int64_t ldq, const vo
       return sums ? launch<kv8::kInt8, kN, true>(map, p, sums, stream) : launch<kv8::kInt8, kN, false>(map, p, sums, stream);
     return sums ? launch<kv8::kE4m3, kN, true>(map, p, sums, stream) : launch<kv8::kE4m3, kN, false>(map, p, sums, stream);
   };
-  return N == 1 ? go(std::integral_constant<int, 1>()) : N == 2 ? go(std::integral_constant<int, 2>())
-                                                               : go(std::integral_constant<int, 4>());
+  return N == 1 ? go(std::integral_constant<int, 1>()) : go(std::integral_constant<int, 2>());
 }
