@@ -303,8 +303,8 @@ int mes_awq_gemv(int epilogue, const void* X, int64_t ldx, const int32_t* qweigh
  *           i of sequence b is token context_lens[b] - (cu_new[b+1] - cu_new[b]) + i
  * D == 128; P = page_size is 16, 32, 64 or 128; num_pages * 2 * Hkv * P < 2^31 rows.
  * max_new: an upper bound on the new tokens of one sequence, known to the host.  Lengths and
- * pages are read on the device; ones that lie outside T, the table or the cache are skipped and
- * record MES_ERR_INVALID as device error.  Sequences must not share pages that a call writes:
+ * pages are read on the device; ones that lie outside T, max_new, the table or the cache are
+ * skipped and record MES_ERR_INVALID as device error.  Sequences must not share pages that a call writes:
  * those of new tokens, and, where a call has sums, every page. */
 
 /* Quantises new keys and values into the cache.  K, V: bf16 rows of pitch ldk / ldv elements,

@@ -83,7 +83,7 @@ struct Params {
   int64_t width;
   const int32_t* cu;
   const int32_t* ctx;
-  int B, T, Hq, Hkv, G, P, page_shift;
+  int B, T, max_new, Hq, Hkv, G, P, page_shift;
   int64_t num_pages;
   float scale;
   __nv_bfloat16* out;
@@ -159,13 +159,13 @@ __device__ __forceinline__ int row_tiles(int n, int G) { return (n * G + kRows -
 struct Seq {
   int r0, n, len;
 };
-// Lengths of a sequence, made safe: rows within [0, T), tokens within the table.
+// Lengths of a sequence, made safe: rows within [0, T), at most max_new, tokens within the table.
 __device__ __forceinline__ Seq sequence(const Params& p, int b) {
   Seq s;
   s.r0 = p.cu[b];
   s.n = p.cu[b + 1] - s.r0;
   s.len = p.ctx[b];
-  if (s.r0 < 0 || s.n < 0 || (int64_t)s.r0 + s.n > p.T || s.len < 0 || s.len > p.width * p.P) {
+  if (s.r0 < 0 || s.n < 0 || (int64_t)s.r0 + s.n > p.T || s.n > p.max_new || s.len < 0 || s.len > p.width * p.P) {
     atomicCAS(&g_err_kv8_attention, 0, MES_ERR_INVALID);
     s.r0 = s.n = s.len = 0;
   }
@@ -173,7 +173,12 @@ __device__ __forceinline__ Seq sequence(const Params& p, int b) {
 }
 
 // First unit of block i's share.
-__device__ __forceinline__ int share(int64_t units, int i, int blocks) { return (int)(units * i / blocks); }
+// It is floor(units i / blocks) without a 64-bit division.
+struct Shares {
+  int blocks, whole, rest;
+  __device__ __forceinline__ Shares(int units, int blocks) : blocks(blocks), whole(units / blocks), rest(units - whole * blocks) {}
+  __device__ __forceinline__ int at(int i) const { return whole * i + (int)((uint32_t)(rest * i) / (uint32_t)blocks); }
+};
 
 // A block's share of the line of units, with row tiles of kRows query rows.
 struct Found {
@@ -253,8 +258,9 @@ struct Line {
     const int grain = p.whole > 0 ? p.whole : 1;     // a multiple of this many units for each block
     const int all = total.with(cost) / grain, blocks = min((int)gridDim.x, all);
     if ((int)blockIdx.x >= blocks) return false;
-    first = share(all, blockIdx.x, blocks) * grain;
-    end = share(all, blockIdx.x + 1, blocks) * grain;
+    const Shares shares(all, blocks);
+    first = shares.at(blockIdx.x) * grain;
+    end = shares.at(blockIdx.x + 1) * grain;
     if (cost > 0) {             // both at once, in odd and even lanes
       const int x = units_before(lane & 1 ? end : first, cost);
       first = __shfl_sync(0xffffffffu, x, 0);
@@ -859,19 +865,22 @@ kv8_join_kernel(const Params p, int grid) {
   // The item begins at u_item of the line, its units are [u0, u1).
   const int u_item = before.with(cost) + item * (units + cost), u0 = u_item + cost, u1 = u0 + units;
   // The blocks whose shares meet [u0, u1).
-  int from = (int)((int64_t)u0 * blocks / all);
-  while (from + 1 < blocks && share(all, from + 1, blocks) <= u0) ++from;
-  while (from > 0 && share(all, from, blocks) > u0) --from;
-  if (share(all, from + 1, blocks) >= u1) return wait();   // not cut
+  const Shares shares(all, blocks);
+  const float each = (float)blocks / (float)all;             // near enough to begin with
+  int from = min((int)(u0 * each), blocks - 1);
+  while (from + 1 < blocks && shares.at(from + 1) <= u0) ++from;
+  while (from > 0 && shares.at(from) > u0) --from;
+  if (shares.at(from + 1) >= u1) return wait();              // not cut
   const int to = [&] {                                     // one past the last of them
-    int i = (int)((int64_t)(u1 - 1) * blocks / all);
-    while (i + 1 < blocks && share(all, i + 1, blocks) < u1) ++i;
-    while (share(all, i, blocks) >= u1) --i;
+    int i = min((int)((u1 - 1) * each), blocks - 1);
+    while (i + 1 < blocks && shares.at(i + 1) < u1) ++i;
+    while (shares.at(i) >= u1) --i;
     return i + 1;
   }();
   const int local = row - tile * kRows;
+  const bool cut = shares.at(from) < u_item;
   // Only the item's first block can have it as its second segment: where it has units before it.
-  auto slot = [&](int i) { return ((int64_t)2 * i + (i == from && share(all, i, blocks) < u_item ? 1 : 0)) * kRows + local; };
+  auto slot = [&](int i) { return ((int64_t)2 * i + (i == from && cut ? 1 : 0)) * kRows + local; };
   wait();                                                  // the partial results are there
   // Each of the W warps takes every W-th partial result; its loads do not wait for one another.
   float mx = -INFINITY, sum = 0.f;
@@ -1101,6 +1110,7 @@ extern "C" int mes_kv8_attention(int dtype, const void* q, int64_t ldq, const vo
   p.ctx = context_lens;
   p.B = (int)B;
   p.T = (int)T;
+  p.max_new = (int)max_new;
   p.Hq = Hq;
   p.Hkv = Hkv;
   p.G = G;

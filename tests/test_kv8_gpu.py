@@ -461,6 +461,8 @@ def test_attention_reports_bad_pages_and_lengths():
     assert _C.take_device_error() == 1
     call(cache.table, _cu([1, 5]), cache.lens)
     assert _C.take_device_error() == 1
+    call(cache.table, _cu([2, 0]), cache.lens)               # more new tokens than max_new
+    assert _C.take_device_error() == 1
 
 
 # ------------------------------------------------------------------------------ evict
