@@ -12,8 +12,8 @@
 // at most two partial results a block (its first and its last segment), joined by a second kernel.
 // The lengths stay on the device.  Where no sequence can be long (the table has room for four units
 // at most), items are dealt whole and there is no second kernel: 256 sequences of 100 to 500 tokens
-// take 51 instead of 71 us.  One of 500 alone takes 10.5 instead of 7.9, but its call, which the
-// host bounds, 14.5 instead of 17.
+// take 51 instead of 71 us.  One of 500 alone takes 10.0 instead of 7.9, but its call, which the
+// host bounds, 10.8 instead of 17.
 //
 // A block is four warps.  Each takes 32 keys of a unit for itself: its own ring of TMA tiles
 // (128-byte swizzle, so the 16-byte reads below meet no bank conflict), its own running maximum

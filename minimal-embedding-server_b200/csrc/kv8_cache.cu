@@ -297,7 +297,7 @@ kv8_read_kernel(const uint8_t* __restrict__ codes, const float* __restrict__ sca
 // 11 and 10 bits, added over the cluster through distributed shared memory; then each warp walks
 // its part of the slice in token order, so the kept indices come out sorted and a tie goes to
 // the lower index.
-// Measured: 8 heads of 100003 tokens 24.5 us, 64 of 4096 11.8 us.  Latency bounds it: lengths, pages and
+// Measured: 8 heads of 100003 tokens 24.5 us, 64 of 4096 10.3 us.  Latency bounds it: lengths, pages and
 // sums are loaded one after the other (5 us), and each pass has two barriers of the cluster (5 us).
 constexpr int kSelThreads = 1024, kBins = 2048, kSelWarps = kSelThreads / 32;
 
