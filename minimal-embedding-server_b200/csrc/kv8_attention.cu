@@ -26,8 +26,13 @@
 // for four steps, and four lanes' V rows are transposed with byte permutes.
 //
 // Scales: a page's K scale multiplies its logits.  Its V scale vs goes into the exponent,
-// p' = exp2(s + log2(vs) - m), with m a running reference near the maximum of s + log2(vs): p'
-// stays within f16 whatever the scales are, and the softmax sum adds p' / vs.
+// p' = exp2(s + log2(vs) - m), with m a running reference near the maximum of s + log2(vs), so that p'
+// stays within f16.  The softmax sum needs exp2(s) alone: it adds p' 2^b / vs, which is exp2(s - (m - b)).
+// The base 2^b is 1 while scales are ordinary (2^-40 to 2^40) and otherwise a power of two near the largest
+// that the warp has seen, so that neither exponent leaves its range whatever the scales are.  V of scale 0, or
+// of less than 2^-60 of the base, counts as 0: its codes are cleared, and its scale is taken as one that
+// does not lift m above what the others need.  When partial results meet, outputs are joined by m and sums
+// by m - b, and the output is multiplied by 2^b at the end.
 //
 // Measured: two sequences of 131072 tokens, 8 kv heads, one query each 93 us (537 MB, 5.8 TB/s, 0.88 of
 // the copy rate); 64 of 100 to 8192 tokens 100 us (0.85).  With 138 query rows for each kv head it
@@ -51,6 +56,9 @@ constexpr int kStageBytes = 2 * kHalfBytes;
 constexpr float kShift = 10.f, kMost = 15.f;
 // Blocks of an SM: registers and shared memory hold three with 8 query rows, two with more.
 constexpr int blocks_per_sm(int N) { return N == 1 ? 3 : 2; }
+// Log2 of the scales around 1 that leave the base there; how far the base may be below a scale otherwise; and
+// how far a scale below the base, before its V counts as 0 (f16 keeps weights down to 2^-35 of the largest).
+constexpr float kOrdinary = 40.f, kBaseStep = 16.f, kBaseRange = 60.f;
 // What beginning an item costs a block, in units of work.  Against 0: 64 ragged sequences of up to
 // 8192 tokens take 100 instead of 105 us.
 constexpr int kSegmentCost = 2;
@@ -68,7 +76,8 @@ struct Smem {
   float qscale[8 * N];                          // logit factor of a row, in the exp2 domain
   int last[8 * N];                              // last visible key of a row
   float2 sc[kWarps][kStages][3];                // factors of a tile's two halves: K scale, log2 and
-                                                // reciprocal of the V scale (-1: V values all 0)
+                                                // reciprocal of the V scale (negative: not an ordinary one)
+  float base[kWarps];                           // the warps' bases, -inf where all V counted as 0
   uint64_t full[kWarps][kStages];
   int2 warp_sum[kWarps];
   int abort;
@@ -88,7 +97,7 @@ struct Params {
   float scale;
   __nv_bfloat16* out;
   float* part_o;        // [blocks][2][8 N][128]
-  float2* part_ml;      // [blocks][2][8 N]
+  float4* part_ml;      // [blocks][2][8 N]: reference of the outputs, that of the sum, the sum
   float* lse;           // [T * Hq] with sums, else null
   float* logits;        // [T * Hq][max_ctx] with sums, else null
   int64_t max_ctx;
@@ -307,7 +316,7 @@ struct Line {
   }
   // Tile `sub` of unit u, in two steps with a load each: its pages, then their scales.
   __device__ __forceinline__ Tile tile(int u, int sub) const {
-    Tile t = {{0, 0}, {0, 0}, 0, 0, make_float2(0.f, 0.f), make_float2(1.f, 1.f)};
+    Tile t = {{0, 0}, {0, 0}, 0, 0, make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
     if (u >= end) return t;
     const Found at = find(u);
     const Seq s = at.s;
@@ -367,11 +376,10 @@ __device__ __forceinline__ void load_tile(const Params& p, const CUtensorMap& ma
     }
   }
 }
-// A tile's factors: K scale, log2 and reciprocal of the V scale.  V codes of scale 0 count as 0, so
-// their factor is free, here 1; the mark is a reciprocal of -1.
-__device__ __forceinline__ void tile_factors(const Tile& t, float2& lv, float2& iv) {
-  lv = make_float2(t.vs.x == 0.f ? 0.f : log2f(t.vs.x), t.vs.y == 0.f ? 0.f : log2f(t.vs.y));
-  iv = make_float2(t.vs.x == 0.f ? -1.f : 1.f / t.vs.x, t.vs.y == 0.f ? -1.f : 1.f / t.vs.y);
+// Log2 of a V scale and its reciprocal, negative where the scale is not an ordinary one.
+__device__ __forceinline__ float2 v_factors(float vs) {
+  const float lv = log2f(vs);
+  return make_float2(lv, fabsf(lv) <= kOrdinary ? 1.f / vs : -1.f);
 }
 // Part `part` of a query row: f16 times a power of two that brings the row's largest value near
 // 2^8, as the B fragments of its four steps; returns the logit factor of the row.  The eight lanes
@@ -476,7 +484,7 @@ __device__ __forceinline__ void weights(const Params& p, float (&S)[N][2][4], fl
     for (int mt = 0; mt < 2; ++mt) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) x[mt][e] = ex2(x[mt][e]);
-      const float inv = fabsf(mt == 0 ? iv.x : iv.y);
+      const float inv = mt == 0 ? iv.x : iv.y;
       l[t][0] = fmaf(x[mt][0] + x[mt][2], inv, l[t][0]);
       l[t][1] = fmaf(x[mt][1] + x[mt][3], inv, l[t][1]);
       const __half2 p0 = __floats2half2_rn(x[mt][0], x[mt][1]), p1 = __floats2half2_rn(x[mt][2], x[mt][3]);
@@ -525,7 +533,11 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
   };
   auto factors = [&](int i) {    // and what goes with it: apart, since the scales arrive later
     if (first + i >= end) return;
-    if ((i & 31) == 0) tile_factors(t_tile, t_lv, t_iv);
+    if ((i & 31) == 0) {
+      const float2 x = v_factors(t_tile.vs.x), y = v_factors(t_tile.vs.y);
+      t_lv = make_float2(x.x, y.x);
+      t_iv = make_float2(x.y, y.y);
+    }
     if (lane == (i & 31)) {
       sh.sc[warp][i % kStages][0] = t_tile.ks;
       sh.sc[warp][i % kStages][1] = t_lv;
@@ -619,6 +631,22 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
       m[t][0] = m[t][1] = -INFINITY;
       l[t][0] = l[t][1] = 0.f;
     }
+    float base = 0.f;             // log2 of the base
+    bool any = false;             // any V that does not count as 0; O is 0 until then
+    int plain_len = s.len;        // tiles that end by it and have ordinary scales need nothing else; -1 with another base
+    auto move_base = [&](float to) {
+      const float d = to - base, alpha = any ? ex2(-d) : 1.f;
+#pragma unroll
+      for (int t = 0; t < N; ++t) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) O[t][i][e] *= alpha;
+        m[t][0] += d;
+        m[t][1] += d;
+      }
+      base = to;
+    };
 
     for (; u < stop; ++u) {
       const int i = u - first, stage = i % kStages;
@@ -629,17 +657,31 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
         phase ^= 1u << stage;
         const uint8_t* kt = sh.ring[warp][stage];
         const uint8_t* vt = kt + kHalfBytes;
-        const float2 ks = sh.sc[warp][stage][0], lv = sh.sc[warp][stage][1], iv = sh.sc[warp][stage][2];
-        if (t0 + kTile > s.len || iv.x < 0.f || iv.y < 0.f) {
-          // V slots past the end hold anything, NaN codes too, and 0 * NaN is NaN; codes of scale 0
+        const float2 ks = sh.sc[warp][stage][0];
+        float2 lv = sh.sc[warp][stage][1], iv = sh.sc[warp][stage][2];
+        if (t0 + kTile > plain_len || iv.x < 0.f || iv.y < 0.f) {
+          const float top = fmaxf(lv.x, lv.y);
+          if (top > -INFINITY) {
+            const float to = fabsf(top) <= kOrdinary ? 0.f : floorf(top);
+            if (any ? top > (base == 0.f ? kOrdinary : base + kBaseStep) : to != base) move_base(to);
+            any = true;
+            plain_len = base == 0.f ? s.len : -1;
+          }
+          // V slots past the end hold anything, NaN codes too, and 0 * NaN is NaN; codes of no scale
           // count as 0.  Lane = slot.
-          if (t0 + lane >= s.len || (lane < 16 ? iv.x : iv.y) < 0.f) {
+          const bool none0 = lv.x < base - kBaseRange, none1 = lv.y < base - kBaseRange;
+          if (t0 + lane >= s.len || (lane < 16 ? none0 : none1)) {
             uint4* row = reinterpret_cast<uint4*>(const_cast<uint8_t*>(vt) + lane * kv8::kD);
 #pragma unroll
             for (int j = 0; j < 8; ++j) row[j] = make_uint4(0, 0, 0, 0);
           }
           mes::fence_proxy_async_smem();      // before the stage is loaded again
           __syncwarp();
+          const float none = base == 0.f ? -kOrdinary : base;
+          lv = make_float2(none0 ? none : lv.x, none1 ? none : lv.y);
+          iv = make_float2(ex2(base - lv.x), ex2(base - lv.y));
+        } else {
+          any = true;
         }
         // ---- S^T = K Q^T: keys 16 mt + key_of(g) and 8 more by rows 2 c and 2 c + 1 ----
         float S[N][2][4];
@@ -741,7 +783,10 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
       a.w = a.w * fm[1] + x.w * ft[1];
     };
     const bool upper = warp >= 2, odd = warp & 1;
+    if (lane == 0) sh.base[warp] = any ? base : -INFINITY;
     __syncthreads();
+    const float most = fmaxf(fmaxf(sh.base[0], sh.base[1]), fmaxf(sh.base[2], sh.base[3]));
+    if (most != -INFINITY && most != base) move_base(most);      // one base for the four
 #pragma unroll
     for (int i = 0; i < 4 * N; ++i) {
       const int j = i + 4 * N;
@@ -794,22 +839,25 @@ kv8_attention_kernel(const __grid_constant__ CUtensorMap map, const Params p) {
       if (whole) {
         const int q = row_base + row, qi = q / p.G;
         const int64_t at = (int64_t)(s.r0 + qi) * p.Hq + h * p.G + q - qi * p.G;
-        const float inv = row_l[e] > 0.f ? 1.f / row_l[e] : row_l[e] == 0.f ? 0.f : row_l[e];      // NaN stays NaN
+        const float half = ex2(0.5f * base);      // 2^base in two steps, either of which may be
+        const float inv = half * (row_l[e] > 0.f ? 1.f / row_l[e] : row_l[e] == 0.f ? 0.f : row_l[e]);     // NaN stays NaN
         uint32_t w[2 * N];
 #pragma unroll
         for (int i = 0; i < 2 * N; ++i)
-          w[i] = mes::pack_bf16x2((e ? part[i].y : part[i].x) * inv, (e ? part[i].w : part[i].z) * inv);
+          w[i] = mes::pack_bf16x2((e ? part[i].y : part[i].x) * inv * half, (e ? part[i].w : part[i].z) * inv * half);
         uint2* dst = reinterpret_cast<uint2*>(p.out + at * kv8::kD + 16 * g + at16);
 #pragma unroll
         for (int i = 0; i < N; ++i) dst[i] = make_uint2(w[2 * i], w[2 * i + 1]);
-        if (kSums && g == 0 && at16 == 0) p.lse[at] = row_m[e] + log2f(row_l[e]);
+        if (kSums && g == 0 && at16 == 0) p.lse[at] = row_m[e] - base + log2f(row_l[e]);
       } else {
         float4* dst = reinterpret_cast<float4*>(p.part_o + ((int64_t)slot * kRows + row) * kv8::kD + 16 * g + at16);
 #pragma unroll
         for (int i = 0; i < N; ++i)
           dst[i] = e ? make_float4(part[2 * i].y, part[2 * i].w, part[2 * i + 1].y, part[2 * i + 1].w)
                      : make_float4(part[2 * i].x, part[2 * i].z, part[2 * i + 1].x, part[2 * i + 1].z);
-        if (g == 0 && at16 == 0) p.part_ml[(int64_t)slot * kRows + row] = make_float2(row_m[e], row_l[e]);
+        if (g == 0 && at16 == 0)
+          p.part_ml[(int64_t)slot * kRows + row] =
+              make_float4(most == -INFINITY ? most : row_m[e], row_m[e] - base, row_l[e], 0.f);
       }
     }
   }
@@ -828,7 +876,7 @@ __global__ void __launch_bounds__(kThreads)
 kv8_join_kernel(const Params p, int grid) {
   constexpr int kRows = 8 * N;
   __shared__ float4 part[kWarps][32];
-  __shared__ float2 part_ml[kWarps];
+  __shared__ float3 part_ml[kWarps];
   if (kSums) asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   // Every block waits for the attention kernel's end before it ends itself, whether it has work or
@@ -882,64 +930,73 @@ kv8_join_kernel(const Params p, int grid) {
   // Only the item's first block can have it as its second segment: where it has units before it.
   auto slot = [&](int i) { return ((int64_t)2 * i + (i == from && cut ? 1 : 0)) * kRows + local; };
   wait();                                                  // the partial results are there
-  // Each of the W warps takes every W-th partial result; its loads do not wait for one another.
-  float mx = -INFINITY, sum = 0.f;
+  // Each of the W warps takes every W-th partial result; its loads do not wait for one another.  Outputs
+  // go by the reference `mx`, sums by `ms`: they differ by the blocks' bases.
+  float mx = -INFINITY, ms = -INFINITY, sum = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto factor = [](float from, float to) { return from == -INFINITY ? 0.f : ex2(from - to); };
   for (int i0 = from + warp % W; i0 < to; i0 += 8 * W) {
-    float2 ml[8];
-    float4 x[8];
+    float4 ml[8], x[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      ml[j] = make_float2(-INFINITY, 0.f);
+      ml[j] = make_float4(-INFINITY, -INFINITY, 0.f, 0.f);
       x[j] = make_float4(0.f, 0.f, 0.f, 0.f);
       if (i0 + j * W < to) {
         ml[j] = p.part_ml[slot(i0 + j * W)];
         x[j] = *reinterpret_cast<const float4*>(p.part_o + slot(i0 + j * W) * kv8::kD + 4 * lane);
       }
     }
-    float now = mx;
+    float now = mx, now_s = ms;
 #pragma unroll
-    for (int j = 0; j < 8; ++j) now = fmaxf(now, ml[j].x);
-    const float keep = mx == -INFINITY ? 0.f : ex2(mx - now);
-    sum *= keep;
+    for (int j = 0; j < 8; ++j) {
+      now = fmaxf(now, ml[j].x);
+      now_s = fmaxf(now_s, ml[j].y);
+    }
+    const float keep = factor(mx, now);
+    sum *= factor(ms, now_s);
     o = make_float4(o.x * keep, o.y * keep, o.z * keep, o.w * keep);
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
-      const float f = ml[j].x == -INFINITY ? 0.f : ex2(ml[j].x - now);
-      sum += f * ml[j].y;
+      const float f = factor(ml[j].x, now);
+      sum += factor(ml[j].y, now_s) * ml[j].z;
       o.x += f * x[j].x;
       o.y += f * x[j].y;
       o.z += f * x[j].z;
       o.w += f * x[j].w;
     }
     mx = now;
+    ms = now_s;
   }
   if (W > 1) {
     part[warp][lane] = o;
-    if (lane == 0) part_ml[warp] = make_float2(mx, sum);
+    if (lane == 0) part_ml[warp] = make_float3(mx, ms, sum);
     __syncthreads();                // W == kWarps: the block's warps have all come here
     if (warp != 0) return;
-    mx = -INFINITY;
+    mx = ms = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < W; ++w) mx = fmaxf(mx, part_ml[w].x);
+    for (int w = 0; w < W; ++w) {
+      mx = fmaxf(mx, part_ml[w].x);
+      ms = fmaxf(ms, part_ml[w].y);
+    }
     sum = 0.f;
     o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < W; ++w) {
-      const float2 ml = part_ml[w];
+      const float3 ml = part_ml[w];
       const float4 x = part[w][lane];
-      const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - mx);
-      sum += f * ml.y;
+      const float f = factor(ml.x, mx);
+      sum += factor(ml.y, ms) * ml.z;
       o.x += f * x.x;
       o.y += f * x.y;
       o.z += f * x.z;
       o.w += f * x.w;
     }
   }
-  const float inv = sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum;
+  const float half = mx == -INFINITY ? 1.f : ex2(0.5f * (mx - ms));      // 2^base in two steps; no reference: o is 0
+  const float inv = half * (sum > 0.f ? 1.f / sum : sum == 0.f ? 0.f : sum);
   *reinterpret_cast<uint2*>(p.out + at * kv8::kD + 4 * lane) =
-      make_uint2(mes::pack_bf16x2(o.x * inv, o.y * inv), mes::pack_bf16x2(o.z * inv, o.w * inv));
-  if (kSums && lane == 0) p.lse[at] = mx + log2f(sum);
+      make_uint2(mes::pack_bf16x2(o.x * inv * half, o.y * inv * half), mes::pack_bf16x2(o.z * inv * half, o.w * inv * half));
+  if (kSums && lane == 0) p.lse[at] = ms + log2f(sum);
 }
 
 // ---- sums[t] += sum over the rows of a kv head of exp2(logit - lse): a thread for four keys, which
@@ -1001,7 +1058,7 @@ Layout layout(int64_t T, int Hq, int N, int64_t max_ctx) {
   const int64_t slots = 2ll * max_blocks(N) * 8 * N;
   w.part_o = 0;
   w.part_ml = w.part_o + slots * kv8::kD * 4;
-  w.lse = up256(w.part_ml + slots * 8);
+  w.lse = up256(w.part_ml + slots * 16);
   w.logits = up256(w.lse + (max_ctx > 0 ? 4 * T * Hq : 0));
   w.bytes = w.logits + 4 * T * Hq * max_ctx;
   return w;
@@ -1120,7 +1177,7 @@ extern "C" int mes_kv8_attention(int dtype, const void* q, int64_t ldq, const vo
   p.scale = scale;
   p.out = (__nv_bfloat16*)out;
   p.part_o = (float*)(ws + w.part_o);
-  p.part_ml = (float2*)(ws + w.part_ml);
+  p.part_ml = (float4*)(ws + w.part_ml);
   p.lse = sums ? (float*)(ws + w.lse) : nullptr;
   p.logits = sums ? (float*)(ws + w.logits) : nullptr;
   p.max_ctx = max_ctx;
