@@ -8,7 +8,8 @@ last-token states, as ``GPUWorker.embed`` does.
 
 A text may be given a budget: when its cache grows past it, the tokens with the smallest accumulated
 attention weight are dropped, for each layer and kv head by itself; the most recent ones stay.
-Positions go on counting from the text's first token.
+Positions go on counting from the text's first token, so a text ends with the model's rotary table: a call that
+would pass it raises ``MesError`` and changes nothing.
 
 Every layer has its own cache and all layers use the same pages, so one block table serves a step.
 Runs of at most 16 new tokens in all take the matrix-vector kernels, as CUDA graphs once their sizes come
@@ -95,6 +96,7 @@ class IncrementalEmbedder:
         self._next = 0
         self.use_cuda_graphs = self.device.type == "cuda" and os.environ.get("MES_CUDA_GRAPHS", "1") != "0"
         self.max_graphs = 32
+        self._positions = layers[0].self_attn.rotary_emb.cos_sin_cache.shape[0] if len(layers) else None
         self._tp_size = layers[0].self_attn.o_proj.tp_size if len(layers) else 1
         self._graphs: collections.OrderedDict[tuple, _StepGraph | None] = collections.OrderedDict()
         self._pool = None
@@ -189,6 +191,9 @@ class IncrementalEmbedder:
         if not texts:
             return torch.empty(0, self.model.norm.hidden_size, dtype=torch.float32, device=self.device)
         counts = [len(t) for t in tokens]
+        end = max(t.position + n for t, n in zip(texts, counts))
+        if self._positions is not None and end > self._positions:
+            raise _C.MesError(f"the model has {self._positions} positions, a text would have {end} tokens")
         need = [max(self._pages_for(t.cached + n) - len(t.pages), 0) for t, n in zip(texts, counts)]
         # Those that eviction copies to are there before anything runs, so that a text is extended whole or not at all.
         self._need(sum(need) + sum(self._pages_for(self.budget) for t, n in zip(texts, counts) if self._over(t.cached + n)))

@@ -200,3 +200,23 @@ def test_incremental_pages_and_launches(rec):
     assert len(emb._free) == 7 and len(emb._texts) == 4
     emb.drop(handles + forks)
     assert sorted(emb._free) == list(range(12)) and not emb._texts
+
+
+def test_texts_end_with_the_rotary_table(rec):
+    """Positions go on counting under a budget; past the table there is no rotation to give."""
+    cfg = synthetic.qwen3_0_6b(num_hidden_layers=1, vocab_size=500, max_position_embeddings=64)
+    emb = IncrementalEmbedder(Qwen3ForCausalLM(MESConfig(model_config=cfg)), num_pages=40, page_size=16, budget=32)
+    (h,), _ = emb.add([np.arange(30)])
+    for _ in range(34):
+        emb.extend([h], [[1]])
+    assert emb._texts[h].position == 64
+    (other,) = emb.fork(h, 1)
+    rec.calls.clear()
+    state = (list(emb._free), list(emb._texts[h].pages), emb.cached_tokens(h))
+    for call in (lambda: emb.extend([h], [[1]]), lambda: emb.extend([other], [[1, 2]]), lambda: emb.add([np.arange(65)]),
+                 lambda: emb.add([[1], np.arange(70)])):
+        with pytest.raises(_C.MesError, match="64 positions"):
+            call()
+        assert rec.calls == []
+    assert (emb._free, emb._texts[h].pages, emb.cached_tokens(h)) == state and set(emb._texts) == {h, other}
+    emb.add([np.arange(64)])
