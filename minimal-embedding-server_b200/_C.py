@@ -699,6 +699,15 @@ def _kv8_workspace(device: int, *sizes: int) -> int:
     return int(lib().mes_kv8_attention_workspace_size(*sizes))
 
 
+def kv8_attention_fits(B: int, max_new: int, num_heads: int, num_kv_heads: int, tokens: int) -> bool:
+    """Whether one ``kv8_attention`` takes ``B`` sequences with at most ``max_new`` new tokens each, over tables with
+    room for ``tokens``: its limits on sequences, rows and units of work (128 keys of eight query rows)."""
+    tiles, units = -(-max_new * (num_heads // num_kv_heads) // 8), -(-tokens // 128) + 2
+    most = 2 ** 31 - 1
+    return (B <= 1024 and B * num_kv_heads <= 65535 and B * max_new * num_heads <= most
+            and B * tiles * num_kv_heads * units <= most)
+
+
 def kv8_attention(q: torch.Tensor, codes: torch.Tensor, scales: torch.Tensor,
                   block_table: torch.Tensor, cu_new: torch.Tensor, context_lens: torch.Tensor,
                   num_heads: int, scale: float, max_new: int, out: torch.Tensor | None = None,

@@ -194,9 +194,29 @@ class IncrementalEmbedder:
         end = max(t.position + n for t, n in zip(texts, counts))
         if self._positions is not None and end > self._positions:
             raise _C.MesError(f"the model has {self._positions} positions, a text would have {end} tokens")
+        parts = self._parts(texts, counts, first)
+        # The pages that new tokens need, and those that eviction copies to, are there before anything runs.
         need = [max(self._pages_for(t.cached + n) - len(t.pages), 0) for t, n in zip(texts, counts)]
-        # Those that eviction copies to are there before anything runs, so that a text is extended whole or not at all.
         self._need(sum(need) + sum(self._pages_for(self.budget) for t, n in zip(texts, counts) if self._over(t.cached + n)))
+        out = [self._run_part(texts[a:b], tokens[a:b], counts[a:b], need[a:b], first) for a, b in parts]
+        return out[0] if len(out) == 1 else torch.cat(out)
+
+    def _parts(self, texts, counts, first: bool) -> list[tuple[int, int]]:
+        """The texts cut into ranges that the cache attention takes in one call."""
+        if not len(self.model.layers) or first and (self.budget is None or self.observe <= 0):
+            return [(0, len(texts))]
+        attn, parts, a, new, tokens = self.model.layers[0].self_attn, [], 0, 0, 0
+        for i, (t, n) in enumerate(zip(texts, counts)):
+            n, c = min(n, self.observe) if first else n, max(self._pages_for(t.cached + n), len(t.pages)) * self.page_size
+            if i > a and not _C.kv8_attention_fits(i + 1 - a, max(new, n), attn.num_heads, attn.num_kv_heads, max(tokens, c)):
+                parts.append((a, i))
+                a, new, tokens = i, 0, 0
+            new, tokens = max(new, n), max(tokens, c)
+            if i == a and not _C.kv8_attention_fits(1, new, attn.num_heads, attn.num_kv_heads, tokens):
+                raise _C.MesError(f"{n} new tokens of a text of {t.cached + n} are more than one call takes")
+        return parts + [(a, len(texts))]
+
+    def _run_part(self, texts, tokens, counts, need, first: bool) -> torch.Tensor:
         pages = self._take(sum(need))
         for t, n in zip(texts, need):
             t.pages += [pages.pop() for _ in range(n)]

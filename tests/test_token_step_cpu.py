@@ -220,3 +220,52 @@ def test_texts_end_with_the_rotary_table(rec):
         assert rec.calls == []
     assert (emb._free, emb._texts[h].pages, emb.cached_tokens(h)) == state and set(emb._texts) == {h, other}
     emb.add([np.arange(64)])
+
+
+def _cached_texts(model, count, tokens=1, **kw):
+    """``count`` texts whose one page is taken, as if ``add`` had run."""
+    emb = IncrementalEmbedder(model, num_pages=4 * count, page_size=16, **kw)
+    handles, _ = emb.add([np.arange(tokens)] * count)
+    return emb, handles
+
+
+@pytest.mark.parametrize("budget", [None, 8])
+def test_more_texts_than_one_attention_call_takes(rec, budget):
+    """1024 sequences are what ``mes_kv8_attention`` takes: longer lists run in parts, in order."""
+    cfg = synthetic.qwen3_0_6b(num_hidden_layers=2, vocab_size=500)
+    model = Qwen3ForCausalLM(MESConfig(model_config=cfg))
+    emb, handles = _cached_texts(model, 1500, tokens=9, budget=budget, observe=2)
+    rec.calls.clear()
+    assert emb.extend(handles, [[1]] * 1500).shape == (1500, cfg.hidden_size)
+    # two parts of two layers, one write and one attention each
+    assert rec.calls.count("mes_kv8_append") == rec.calls.count("mes_kv8_attention") == 4
+    assert all(emb._texts[h].position == 10 for h in handles)
+    emb.drop(handles)
+    assert sorted(emb._free) == list(range(6000))
+
+
+def test_a_step_past_what_the_attention_counts(rec):
+    """The attention counts its units in 32 bits: a call past that is split, a single text past it refused,
+    and the refusal changes nothing."""
+    assert _C.kv8_attention_fits(1024, 1, 16, 8, 4096) and not _C.kv8_attention_fits(1025, 1, 16, 8, 4096)
+    assert _C.kv8_attention_fits(4, 60000, 16, 8, 65536) and not _C.kv8_attention_fits(64, 60000, 16, 8, 65536)
+    cfg = synthetic.qwen3_0_6b(num_hidden_layers=1, vocab_size=500)
+    emb, handles = _cached_texts(Qwen3ForCausalLM(MESConfig(model_config=cfg)), 3)
+    rec.calls.clear()
+    fits = []
+    real = _C.kv8_attention_fits
+
+    def tight(B, max_new, heads, kv_heads, tokens):
+        fits.append((B, max_new, heads, kv_heads, tokens))
+        return real(B, max_new, heads, kv_heads, tokens) and B * max_new <= 6
+    _C.kv8_attention_fits = tight
+    try:
+        emb.extend(handles, [[1] * 4, [2] * 3, [3]])           # 4 | 3, 1 (two texts of at most 3)
+        assert rec.calls.count("mes_kv8_append") == 2
+        rec.calls.clear()
+        state = list(emb._free), [(list(emb._texts[h].pages), emb.cached_tokens(h)) for h in handles]
+        with pytest.raises(_C.MesError, match="one call"):
+            emb.extend(handles, [[1], [2], [3] * 7])
+        assert rec.calls == [] and state == (list(emb._free), [(list(emb._texts[h].pages), emb.cached_tokens(h)) for h in handles])
+    finally:
+        _C.kv8_attention_fits = real
