@@ -327,7 +327,8 @@ int mes_kv8_read(int dtype, const void* codes, const float* scales, const int32_
 
 /* Causal grouped-query attention of the new tokens over the cache (their own keys and values
  * included, so append first).  q: bf16 rows of pitch ldq elements, Hq heads of D, Hq % Hkv == 0;
- * out: bf16 [T][Hq * D].  A token that sees nothing gives zeros.  Scales may be anything finite; values of
+ * out: bf16 [T][Hq * D].  A token that sees nothing gives zeros; the rows of a sequence that is skipped are not
+ * written.  Scales may be anything finite; values of
  * a page whose V scale is less than 2^-60 of that of another page of the sequence may count as 0.  With sums, every cached
  * token's weight, summed over the new tokens and the query heads of its kv head, is added to its
  * sum.  At most 1024 sequences.  workspace: 256-byte aligned, of

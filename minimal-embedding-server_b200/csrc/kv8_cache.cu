@@ -154,7 +154,7 @@ __global__ void __launch_bounds__(Shape<P>::kThreads)
 kv8_append_kernel(const __nv_bfloat16* __restrict__ Kn, int64_t ldk, const __nv_bfloat16* __restrict__ Vn,
                   int64_t ldv, uint8_t* codes, float* scales, float* sums,
                   const int32_t* __restrict__ table, int64_t width, const int32_t* __restrict__ cu,
-                  const int32_t* __restrict__ ctx, int64_t T, int max_pages, int Hkv,
+                  const int32_t* __restrict__ ctx, int64_t T, int max_new, int max_pages, int Hkv,
                   int64_t num_pages) {
   using Run = Shape<P>;
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -165,13 +165,11 @@ kv8_append_kernel(const __nv_bfloat16* __restrict__ Kn, int64_t ldk, const __nv_
   const int run = blockIdx.y * Run::kRuns + warp / Run::kRunWarps;
   const int side = run >= Hkv, h = run - side * Hkv;
   const int r0 = cu[b], n = cu[b + 1] - r0, len = ctx[b], start = len - n;
-  const bool sane = r0 >= 0 && n >= 0 && start >= 0 && r0 + (int64_t)n <= T && (int64_t)len <= width * P;
+  // A sequence with more new tokens than max_new is not written at all, as the attention skips it.
+  const bool sane = r0 >= 0 && n >= 0 && n <= max_new && start >= 0 && r0 + (int64_t)n <= T && (int64_t)len <= width * P;
   const int p = sane ? start / P + j : 0;
   bool ok = run < 2 * Hkv && n > 0 && sane && (int64_t)p * P < len;
-  if (threadIdx.x == 0 && blockIdx.y == 0) {
-    // A sequence with more new tokens than the grid has pages for is an error of the caller.
-    if (!sane || (j == 0 && n > 0 && (len - 1) / P - start / P >= max_pages)) record(MES_ERR_INVALID);
-  }
+  if (!sane && threadIdx.x == 0 && blockIdx.y == 0) record(MES_ERR_INVALID);
   // The page's slots [old, end) are new; this lane has the even or odd rows of the warp's.
   const int old = max(start - p * P, 0), end = ok ? min(len - p * P, P) : 0;
   const int slot0 = warp % Run::kRunWarps * kRows + (lane >> 4), col = (lane & 15) * 8;
@@ -607,7 +605,7 @@ extern "C" int mes_kv8_append(int dtype, const void* K, int64_t ldk, const void*
     auto kernel = dtype == kv8::kInt8 ? kv8_append_kernel<kv8::kInt8, P> : kv8_append_kernel<kv8::kE4m3, P>;
     kernel<<<grid, Run::kThreads, 0, (cudaStream_t)stream>>>(
         (const __nv_bfloat16*)K, ldk, (const __nv_bfloat16*)V, ldv, (uint8_t*)codes, scales, sums,
-        block_table, table_width, cu_new, context_lens, T, (int)pages, Hkv, num_pages);
+        block_table, table_width, cu_new, context_lens, T, (int)max_new, (int)pages, Hkv, num_pages);
     return mes_host::from_cuda(cudaGetLastError());
   });
 }

@@ -612,3 +612,27 @@ def test_empty_batches():
     before = cache.codes.clone()
     _C.kv8_append(none[:, :2 * D], none[:, :2 * D], cache.codes, cache.scales, cache.table, _cu([0]), cache.lens, max_new=0)
     assert torch.equal(cache.codes.view(torch.int8), before.view(torch.int8))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("news,max_new", [([5, 1, 2], 2), ([1, 100, 2], 2), ([70, 70, 3], 69), ([2, 2, 2], 1)])
+def test_append_skips_more_new_tokens_than_max_new(kind, page, news, max_new):
+    """Whether they would fit the pages that the call reckons with or not: the sequence's pages stay as they are, the
+    others are written, and the call is recorded."""
+    ctx, hkv = [8 + news[0], 150, 40], 2
+    made = [Cache(kind, page, hkv, ctx).fill() for _ in range(2)]
+    g = torch.Generator().manual_seed(4)
+    k, v = ((torch.randn(sum(news), hkv * D, generator=g) * 3).to(torch.bfloat16).to(DEV) for _ in range(2))
+    got, want = made
+    _C.kv8_append(k, v, got.codes, got.scales, got.table, _cu(news), got.lens, max_new=max_new, sums=got.sums)
+    assert _C.take_device_error() == 1
+    r0 = 0
+    for b, n in enumerate(news):
+        if n <= max_new:
+            _C.kv8_append(k[r0:r0 + n], v[r0:r0 + n], want.codes, want.scales, want.table[b:b + 1], _cu([n]),
+                          want.lens[b:b + 1], max_new=n, sums=want.sums)
+        r0 += n
+    assert _C.take_device_error() == 0
+    for a, b in ((got.codes.view(torch.int8), want.codes.view(torch.int8)), (got.scales, want.scales), (got.sums, want.sums)):
+        assert torch.equal(a.nan_to_num(nan=-1) if a.is_floating_point() else a, b.nan_to_num(nan=-1) if b.is_floating_point() else b)
