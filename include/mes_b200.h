@@ -351,7 +351,8 @@ int mes_kv8_attention(int dtype, const void* q, int64_t ldq, const void* codes,
  * sequences' present pages.  A new page's scale is the largest of its tokens' scales; a token
  * whose own scale is smaller becomes rne(code * own / scale).  Slots past the last token hold
  * code 0.  kept: i32 [B][Hkv][keep], the tokens kept (-1 past the end); new_lens: i32 [B],
- * min(context_lens, keep).  A sequence of at most `keep` tokens is copied whole. */
+ * min(context_lens, keep).  A sequence of at most `keep` tokens is copied whole; one
+ * whose length lies outside the table counts as empty. */
 int mes_kv8_evict(int dtype, void* codes, float* scales, float* sums,
                   const int32_t* block_table, int64_t table_width, const int32_t* context_lens,
                   int64_t B, const int32_t* new_table, int64_t new_width, int64_t keep,

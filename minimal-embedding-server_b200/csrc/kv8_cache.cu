@@ -335,7 +335,7 @@ kv8_select_kernel(const float* __restrict__ sums, const int32_t* __restrict__ ta
   int len = ctx[b];
   if (len < 0 || len > room) {
     if (tid == 0) record(MES_ERR_INVALID);
-    len = len < 0 ? 0 : static_cast<int>(room);
+    len = 0;
   }
   int32_t* out = kept + (int64_t)item * keep;
   const int left = min(len, keep);

@@ -636,3 +636,26 @@ def test_append_skips_more_new_tokens_than_max_new(kind, page, news, max_new):
     assert _C.take_device_error() == 0
     for a, b in ((got.codes.view(torch.int8), want.codes.view(torch.int8)), (got.scales, want.scales), (got.sums, want.sums)):
         assert torch.equal(a.nan_to_num(nan=-1) if a.is_floating_point() else a, b.nan_to_num(nan=-1) if b.is_floating_point() else b)
+
+
+def test_evict_counts_a_length_outside_the_table_as_nothing():
+    """It is recorded, keeps no token and has empty new pages; the other sequences are not affected."""
+    ctx, keep, page = [100, 90, 80], 40, 16
+    for bad in (-1, 7 * page + 1, 2 ** 31 - 1):
+        cache = Cache(torch.int8, page, 2, ctx, extra=9).fill()
+        used = set(cache.table[cache.table >= 0].tolist())
+        new_table = torch.tensor([p for p in range(cache.num_pages) if p not in used], dtype=torch.int32, device=DEV).view(3, 3)
+        lens = cache.lens.clone()
+        want, want_lens = _C.kv8_evict(cache.codes, cache.scales, cache.sums, cache.table, lens, new_table, keep, 8)
+        pages = [t.clone() for t in (cache.codes, cache.scales, cache.sums)]
+        assert _C.take_device_error() == 0
+        lens[1] = bad
+        got, got_lens = _C.kv8_evict(cache.codes, cache.scales, cache.sums, cache.table, lens, new_table, keep, 8)
+        assert _C.take_device_error() == 1
+        assert got_lens.tolist() == [40, 0, 40] and want_lens.tolist() == [40, 40, 40]
+        assert (got[1] == -1).all() and torch.equal(got[[0, 2]], want[[0, 2]])
+        empty = new_table[1].long()
+        for a, b in zip((cache.codes, cache.scales, cache.sums), pages):
+            assert (a[empty] == 0).all()
+            b[empty] = 0
+            assert torch.equal(a.nan_to_num(nan=-1) if a.is_floating_point() else a, b.nan_to_num(nan=-1) if b.is_floating_point() else b)
