@@ -159,6 +159,10 @@ class IncrementalEmbedder:
         """``count`` new texts that begin with what ``handle`` has cached (copied, since the pages
         of a text are written as it grows)."""
         text, out = self._texts[handle], []
+        if count < 0:
+            raise _C.MesError(f"a text is forked into some others, not {count}")
+        if count == 0:
+            return out
         pages = self._take(len(text.pages) * count)
         src = torch.as_tensor(text.pages, device=self.device).repeat(count)
         dst = torch.as_tensor(pages, device=self.device)

@@ -269,3 +269,15 @@ def test_a_step_past_what_the_attention_counts(rec):
         assert rec.calls == [] and state == (list(emb._free), [(list(emb._texts[h].pages), emb.cached_tokens(h)) for h in handles])
     finally:
         _C.kv8_attention_fits = real
+
+
+def test_fork_into_no_texts(rec):
+    cfg = synthetic.qwen3_0_6b(num_hidden_layers=1, vocab_size=500)
+    emb = IncrementalEmbedder(Qwen3ForCausalLM(MESConfig(model_config=cfg)), num_pages=4, page_size=16)
+    (h,), _ = emb.add([np.arange(20)])
+    assert emb.fork(h, 0) == [] and len(emb._free) == 2 and set(emb._texts) == {h}
+    with pytest.raises(_C.MesError):
+        emb.fork(h, -1)
+    with pytest.raises(_C.MesError):
+        emb.fork(h, 2)
+    assert len(emb._free) == 2 and set(emb._texts) == {h}
