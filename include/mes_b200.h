@@ -284,8 +284,9 @@ int mes_awq_gemm_on_panel(int epilogue, const void* X, int64_t ldx, const void* 
  * mes_awq_gemm_ws: 0 Y bf16 [M, N] = X W (+ bias), 1 Y f32 [M, N] += X W (+ bias), 2 Y bf16
  * [M, N/2] = silu(gate) * up with gate and up columns interleaved in blocks of 16 (bias NULL).
  * W = (q - z) * s is used exactly (mes_awq_gemm rounds it to bf16 first) for |X| < 2^67; larger
- * values overflow to infinity or NaN.  fp32 accumulation in a fixed order.  X: bf16 [M, K], pitch ldx elements; qweight_mes, qzeros, scales, bias as for
- * mes_awq_gemm.  group_size 32, 64 or 128; K % 128 == 0; N % 8 == 0 (N % 32 == 0 for
+ * values overflow to infinity or NaN.  fp32 accumulation in a fixed order; sums are kept in multiples of
+ * 2^-76, so values of |X| below 2^-53 lose bits and below 2^-80 vanish.  X: bf16 [M, K], pitch ldx elements;
+ * qweight_mes, qzeros, scales, bias as for mes_awq_gemm.  group_size 32, 64 or 128; K % 128 == 0; N % 8 == 0 (N % 32 == 0 for
  * epilogue 2); ldx % 8 == 0.  X and qweight_mes 16-byte aligned, scales 8, qzeros 4, Y to its
  * elements.  M = 0 does nothing; M > 16 is MES_ERR_INVALID. */
 int mes_awq_gemv(int epilogue, const void* X, int64_t ldx, const int32_t* qweight_mes,

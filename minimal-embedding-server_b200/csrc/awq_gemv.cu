@@ -20,7 +20,9 @@
 // taking the codes out of their words, so they are used where they lie: masked out of a word, a
 // code at bits 0-3 or 4-7 of a half is the bf16 number q 2^-133 or q 2^-129 (bf16 is linear from
 // zero up to 2^-125), so one shift and four masks make eight operands.  X is multiplied by 2^60 or
-// 2^56 to meet them, which is exact for |x| < 2^67, and the result by 2^73.
+// 2^56 to meet them, which is exact for |x| < 2^67, and the result by 2^73.  A sum is then a multiple of
+// 2^-76, fp32's least number times 2^73: values of x below 2^-53 lose bits, which norms' and activations' rows
+// have next to none of.
 //
 // Measured: 8 rows of 4096 x 24576 with silu 16.2 us (52 MB, 3.2 TB/s, half of the copy rate: the
 // integer pipe that masks the codes is 45% busy, and 384 blocks share 148 SMs unevenly); 1 row of

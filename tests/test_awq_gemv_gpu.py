@@ -175,3 +175,27 @@ def test_refusals():
                 lambda: _C.awq_gemv(torch.zeros(2, 260, dtype=torch.bfloat16, device=DEV)[:, 4:], *wt)):
         with pytest.raises(_C.MesError):
             bad()
+
+
+def test_rows_of_any_size():
+    """A power of two on x is one on the result, bit for bit, where nothing leaves fp32's range.  Small sums are kept to
+    2^-76: K / 16 + 2 K / group roundings for each scale, one for each group and row of sums."""
+    K, N, M, group = 512, 72, 3, 128
+    wt, w = _weights(K, N, group, 13)
+    x = _x(M, K, 5)
+    x[x.abs() < 2.0 ** -8] = 1.0
+    base = _C.awq_gemv_residual(x.to(DEV), *wt, torch.zeros(M, N, device=DEV))
+    for e in (-28, -20, 40, 64):
+        got = _C.awq_gemv_residual((x * 2.0 ** e).to(DEV), *wt, torch.zeros(M, N, device=DEV))
+        # Sums of q x are multiples of 2^(e - 15 - 73), their products with a scale (11 bits from 2^-9 on, or the least,
+        # 2^-24) of 2^(e - 107) and 2^(e - 112): for e = -28 and -20 no bit is below 2^-149.
+        if e < -20:
+            assert torch.equal(got[:, 3:], base[:, 3:] * 2.0 ** e)
+        else:
+            assert torch.equal(got, base * 2.0 ** e)
+    for e in (-60, -70, -90):
+        small = x * 2.0 ** e
+        got = _C.awq_gemv_residual(small.to(DEV), *wt, torch.zeros(M, N, device=DEV)).double().cpu().numpy()
+        y, rel = _expect(small, w, group)
+        most = 1.0 * (K / 16 + 2 * K / group) + K / group + 16          # the largest scale is 1
+        assert (np.abs(got - y) <= rel + most * 2.0 ** -76).all(), e
