@@ -659,3 +659,63 @@ def test_evict_counts_a_length_outside_the_table_as_nothing():
             assert (a[empty] == 0).all()
             b[empty] = 0
             assert torch.equal(a.nan_to_num(nan=-1) if a.is_floating_point() else a, b.nan_to_num(nan=-1) if b.is_floating_point() else b)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("page", [16, 32])
+def test_values_through_many_evictions(kind, page):
+    """A window that slides over a stream.  A value is rounded when it is written, each time its page's scale
+    grows and each time a compaction changes its scale, and scales never shrink on the way, so int8 values are
+    within half a step of the present scale for each of those.  An e4m3 rounding is within 2^-4 of the present value
+    or 2^-10 of the scale, and the value itself drifts by no more than those."""
+    hkv, keep, rounds = 2, 48, 40
+    per = -(-keep // page)
+    pool = list(range(2 * per + 6))
+    cache = Cache(kind, page, hkv, [1], extra=len(pool))
+    g = torch.Generator().manual_seed(21)
+    true, times, scale = (np.zeros((2, hkv, 0, D)), np.zeros((2, hkv, 0)), np.zeros((2, hkv, 0)))
+    pages, most, rounded = [], 0, 0
+
+    def present(pages, n):
+        s = cache.scales[torch.tensor(pages, device=DEV)].double().cpu().numpy()      # [pages, 2, hkv]
+        return np.repeat(s.transpose(1, 2, 0), page, 2)[:, :, :n]
+    cache.sums.zero_()
+    for r in range(rounds):
+        m = int(torch.randint(1, 20, (1,), generator=g))
+        new = torch.randn(2, m, hkv * D, generator=g) * torch.exp(torch.randn(1, m, 1, generator=g))
+        new = new.to(torch.bfloat16)
+        n = true.shape[2] + m
+        while len(pages) * page < n:
+            pages.append(pool.pop())
+        table = torch.tensor([pages], dtype=torch.int32, device=DEV)
+        lens = torch.tensor([n], dtype=torch.int32, device=DEV)
+        _C.kv8_append(new[0].to(DEV), new[1].to(DEV), cache.codes, cache.scales, table, _cu([m]), lens, max_new=m, sums=cache.sums)
+        now = present(pages, n)
+        assert (now[:, :, :n - m] >= scale).all()
+        times = np.concatenate([times + (now[:, :, :n - m] != scale), np.ones((2, hkv, m))], 2)
+        true = np.concatenate([true, new.double().numpy().reshape(2, m, hkv, D).transpose(0, 2, 1, 3)], 2)
+        scale = now
+        if n > keep:
+            to = [pool.pop() for _ in range(per)]
+            kept, _ = _C.kv8_evict(cache.codes, cache.scales, cache.sums, table, lens,
+                                   torch.tensor([to], dtype=torch.int32, device=DEV), keep, keep)
+            assert torch.equal(kept[0, 0], torch.arange(n - keep, n, dtype=torch.int32, device=DEV))
+            pool += pages
+            pages, n = to, keep
+            true, times, scale = true[:, :, -keep:], times[:, :, -keep:], scale[:, :, -keep:]
+            now = present(pages, n)
+            assert (now >= scale).all()
+            times, scale = times + (now != scale), now
+            rounded += 1
+        p = torch.tensor(pages, device=DEV)
+        codes = cache.codes.view(torch.int8)[p].view(kind).float().double().cpu().numpy()
+        got = (codes * cache.scales[p].double().cpu().numpy()[..., None, None]).transpose(1, 2, 0, 3, 4).reshape(2, hkv, -1, D)[:, :, :n]
+        t, s = times[..., None], scale[..., None]
+        if kind == torch.int8:
+            bound = 0.5 * s * t
+        else:
+            bound = t * ((1 + 2.0 ** -4) ** t * np.abs(true) / 16 + s * 2.0 ** -10 * (1 + 2.0 ** -4) ** t)
+        assert (np.abs(got - true) <= bound * (1 + 1e-4)).all(), r
+        most = max(most, int(times.max()))
+    # it reaches what it is about: many compactions, values rounded more than twice again
+    assert rounded > 20 and most > 3 and _C.take_device_error() == 0
