@@ -508,6 +508,8 @@ struct PCfg {
   static_assert(kTmemNeed <= 512, "TMEM budget");
   static_assert(kSBytes == 256 && kZBytes == 64 && kWStage % 128 == 0, "stage layout");
   static_assert(BT % 16 == 0 && BT <= 256 && kXStage % 1024 == 0, "tile");
+  // A set waits by the parity of its stages' barriers, so it has to see every phase of them.
+  static_assert(SST % SETS == 0 && kASlots % SETS == 0, "a stage always goes to the same set");
 };
 
 template <int BT, int SST, int AST, int EPI, int SETS>
@@ -819,6 +821,9 @@ awq_gemm_persistent_kernel(const __grid_constant__ CUtensorMap map_x,
 //                          loads.  Fused: waited for by the even CTA's dequant warps, so
 //                          the MMA's wait on afull covers it; PANEL: waited for by the MMA;
 //   full_w[s]  (each CTA)  fused only: the CTA's weight words, scales and zeros landed;
+//   Fused, these two have one barrier for each stage and set (index it % FST): the stages do not divide by the sets,
+//   so a set meets a stage every second time only, and a wait by the parity of the stage's own barrier
+//   would also pass while the copies of the time between are in flight;
 //   afull[s]   (even CTA)  fused only: A rows of both CTAs written (4 dequant warps of
 //                          each CTA arrive per set);
 //   empty[s]   (each CTA)  the stage's MMAs done (commit multicast to both CTAs);
@@ -835,6 +840,7 @@ struct QCfg {
   static constexpr int SETS = PANEL ? 0 : 2;
   // The panel variant's stages have no weight words, which leaves room for one more stage.
   static constexpr int SST = PANEL ? 6 : 5;
+  static constexpr int FST = PANEL ? SST : SETS * SST;   // barriers of landed copies: a set sees every phase of its own
   static constexpr int kDqWarps = 4 * SETS;
   static constexpr int kEpiWarps = 8;
   static constexpr int kThreads = (2 + kDqWarps + kEpiWarps) * 32;
@@ -858,7 +864,7 @@ struct QCfg {
   static constexpr int kOffBar = kOffOut + kEpiWarps * kOutBuf;
   static constexpr int kSmem = kOffBar + 512 + 1024;
   static_assert(kSmem <= 232448, "shared memory budget");
-  static_assert((4 * SST + 5) * 8 + 8 <= 512, "barrier area");
+  static_assert((2 * FST + 2 * SST + 5) * 8 + 8 <= 512, "barrier area");
   static_assert(kSBytes == 256 && kZBytes == 64 && kWStage % 128 == 0, "stage layout");
   static_assert(kXStage % 1024 == 0 && kAStage % 1024 == 0, "swizzle atoms");
 };
@@ -902,7 +908,7 @@ awq_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x,
                      const __nv_bfloat16* __restrict__ bias, float* __restrict__ R, int64_t ldr,
                      int M, int N, int K, int band, int full, int num_items, int res_tma) {
   using C = QCfg<EPI, PANEL>;
-  constexpr int SST = C::SST;
+  constexpr int SST = C::SST, FST = C::FST;
   constexpr uint32_t kTmemCols = 512;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>(
@@ -912,11 +918,11 @@ awq_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x,
   uint8_t* wst = smem + C::kOffW;
   __nv_bfloat16* outbuf = reinterpret_cast<__nv_bfloat16*>(smem + C::kOffOut);
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + C::kOffBar);
-  uint64_t* full_x = bars;              // [SST]
-  uint64_t* full_w = bars + SST;        // [SST]
-  uint64_t* afull = bars + 2 * SST;     // [SST]
-  uint64_t* empty = bars + 3 * SST;     // [SST]
-  uint64_t* acc_full = bars + 4 * SST;  // [2]
+  uint64_t* full_x = bars;              // [FST]
+  uint64_t* full_w = full_x + FST;      // [FST]
+  uint64_t* afull = full_w + FST;       // [SST]
+  uint64_t* empty = afull + SST;        // [SST]
+  uint64_t* acc_full = empty + SST;     // [2]
   uint64_t* acc_empty = acc_full + 2;   // [2]
   uint64_t* drain = acc_empty + 2;      // [1]
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
@@ -930,9 +936,11 @@ awq_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x,
   const int num_t = (M + C::kTileT - 1) / C::kTileT;
 
   if (threadIdx.x == 0) {
+    for (int f = 0; f < FST; ++f) {
+      mes::mbar_init(&full_x[f], 1);
+      mes::mbar_init(&full_w[f], 1);
+    }
     for (int s = 0; s < SST; ++s) {
-      mes::mbar_init(&full_x[s], 1);
-      mes::mbar_init(&full_w[s], 1);
       mes::mbar_init(&afull[s], 8);
       mes::mbar_init(&empty[s], 1);
     }
@@ -975,24 +983,24 @@ awq_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x,
         const int n0 = pi.f * C::kTileN + (int)rank * kBN;
         const int t0 = pi.t0 + (int)rank * (pi.ntok / 2);
         for (int kb = 0; kb < nk; ++kb, ++it) {
-          const int s = it % SST;
+          const int s = it % SST, f = it % FST;
           if (it >= SST &&
               !mes::mbar_wait(&empty[s], ((it / SST) & 1) ^ 1, abort_flag, &g_err_gemm, MES_ERR_TIMEOUT)) {
             ok = false;
             break;
           }
           if constexpr (PANEL) {
-            if (rank == 0) mes::mbar_arrive_expect_tx(&full_x[s], 2 * (C::kXStage + C::kAStage));
-            mes::tma_load_2d_pair(as + s * C::kAStage, &map_w, full_x0 + 8 * s, kb * kBK, n0);
-            mes::tma_load_2d_pair(xs + s * C::kXStage, &map_x, full_x0 + 8 * s, kb * kBK, t0);
+            if (rank == 0) mes::mbar_arrive_expect_tx(&full_x[f], 2 * (C::kXStage + C::kAStage));
+            mes::tma_load_2d_pair(as + s * C::kAStage, &map_w, full_x0 + 8 * f, kb * kBK, n0);
+            mes::tma_load_2d_pair(xs + s * C::kXStage, &map_x, full_x0 + 8 * f, kb * kBK, t0);
           } else {
-            if (rank == 0) mes::mbar_arrive_expect_tx(&full_x[s], 2 * C::kXStage);
-            mes::tma_load_2d_pair(xs + s * C::kXStage, &map_x, full_x0 + 8 * s, kb * kBK, t0);
+            if (rank == 0) mes::mbar_arrive_expect_tx(&full_x[f], 2 * C::kXStage);
+            mes::tma_load_2d_pair(xs + s * C::kXStage, &map_x, full_x0 + 8 * f, kb * kBK, t0);
             uint8_t* w = wst + s * C::kWStage;
-            mes::mbar_arrive_expect_tx(&full_w[s], C::kWBytes + C::kSBytes + C::kZBytes);
-            mes::tma_load_2d(w, &map_w, &full_w[s], n0, kb * (kBK / 8));
-            mes::tma_load_2d(w + C::kWBytes, &map_s, &full_w[s], n0, kb / 2);
-            mes::tma_load_2d(w + C::kWBytes + 256, &map_z, &full_w[s], n0 / 8, kb / 2);
+            mes::mbar_arrive_expect_tx(&full_w[f], C::kWBytes + C::kSBytes + C::kZBytes);
+            mes::tma_load_2d(w, &map_w, &full_w[f], n0, kb * (kBK / 8));
+            mes::tma_load_2d(w + C::kWBytes, &map_s, &full_w[f], n0, kb / 2);
+            mes::tma_load_2d(w + C::kWBytes + 256, &map_z, &full_w[f], n0 / 8, kb / 2);
           }
         }
       }
@@ -1002,8 +1010,8 @@ awq_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x,
         // copies.  (The cluster barrier at the end keeps the odd CTA until then.)
         const uint64_t tstart = mes::globaltimer_ns();
         for (int i = it - SST < 0 ? 0 : it - SST; i < it; ++i) {
-          while (((rank == 0 && !mes::mbar_try_wait(&full_x[i % SST], (i / SST) & 1)) ||
-                  (!PANEL && !mes::mbar_try_wait(&full_w[i % SST], (i / SST) & 1))) &&
+          while (((rank == 0 && !mes::mbar_try_wait(&full_x[i % FST], (i / FST) & 1)) ||
+                  (!PANEL && !mes::mbar_try_wait(&full_w[i % FST], (i / FST) & 1))) &&
                  mes::globaltimer_ns() - tstart < mes::kWaitLimitNs) {
           }
         }
@@ -1030,7 +1038,7 @@ awq_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x,
         for (int kb = 0; kb < nk; ++kb, ++it) {
           const int s = it % SST;
           // Fused: afull implies full_x (the even CTA's dequant warps wait for both X halves
-          // before arriving), so one barrier check per k-step suffices.
+          // before arriving), so one barrier check per k-step suffices.  (FST == SST for a panel.)
           uint64_t* ready = PANEL ? &full_x[s] : &afull[s];
           if (!mes::mbar_wait(ready, (it / SST) & 1, abort_flag, &g_err_gemm, MES_ERR_TIMEOUT)) {
             ok = false;
@@ -1069,11 +1077,12 @@ awq_gemm_pair_kernel(const __grid_constant__ CUtensorMap map_x,
         for (int kb = 0; kb < nk; ++kb, ++it) {
           if (it % C::SETS != set) continue;
           const int s = it % SST;
+          const int f = it % FST;
           // The A slot of a stage is free once the stage's weights landed again: the
           // producer refills a stage only after its MMAs completed.
-          if (!mes::mbar_wait_warp(&full_w[s], (it / SST) & 1, abort_flag, &g_err_gemm, MES_ERR_TIMEOUT) ||
+          if (!mes::mbar_wait_warp(&full_w[f], (it / FST) & 1, abort_flag, &g_err_gemm, MES_ERR_TIMEOUT) ||
               (rank == 0 &&
-               !mes::mbar_wait_warp(&full_x[s], (it / SST) & 1, abort_flag, &g_err_gemm, MES_ERR_TIMEOUT))) {
+               !mes::mbar_wait_warp(&full_x[f], (it / FST) & 1, abort_flag, &g_err_gemm, MES_ERR_TIMEOUT))) {
             ok = false;
             break;
           }
