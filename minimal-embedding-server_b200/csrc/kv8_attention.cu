@@ -379,7 +379,7 @@ __device__ __forceinline__ void load_tile(const Params& p, const CUtensorMap& ma
 // Log2 of a V scale and its reciprocal, negative where the scale is not an ordinary one.
 __device__ __forceinline__ float2 v_factors(float vs) {
   const float lv = log2f(vs);
-  return make_float2(lv, fabsf(lv) <= kOrdinary ? 1.f / vs : -1.f);
+  return make_float2(lv, fabsf(lv) <= kOrdinary ? ex2(-lv) : -1.f);
 }
 // Part `part` of a query row: f16 times a power of two that brings the row's largest value near
 // 2^8, as the B fragments of its four steps; returns the logit factor of the row.  The eight lanes
