@@ -12,8 +12,8 @@
 // at most two partial results a block (its first and its last segment), joined by a second kernel.
 // The lengths stay on the device.  Where no sequence can be long (the table has room for four units
 // at most), items are dealt whole and there is no second kernel: 256 sequences of 100 to 500 tokens
-// take 51 instead of 71 us.  One of 500 alone takes 10.0 instead of 7.9, but its call, which the
-// host bounds, 10.8 instead of 17.
+// take 58 instead of 63 us.  One of 500 alone takes 10.1 instead of 8.8, but its call, which the
+// host bounds, 12.3 instead of 15.6.
 //
 // A block is four warps.  Each takes 32 keys of a unit for itself: its own ring of TMA tiles
 // (128-byte swizzle, so the 16-byte reads below meet no bank conflict), its own running maximum
@@ -34,9 +34,9 @@
 // does not lift m above what the others need.  When partial results meet, outputs are joined by m and sums
 // by m - b, and the output is multiplied by 2^b at the end.
 //
-// Measured: two sequences of 131072 tokens, 8 kv heads, one query each 93 us (537 MB, 5.8 TB/s, 0.88 of
-// the copy rate); 64 of 100 to 8192 tokens 100 us (0.85).  With 138 query rows for each kv head it
-// comes to 250 TFLOP/s (8 sequences of 16384 tokens): two warps a scheduler, which is what the
+// Measured: two sequences of 131072 tokens, 8 kv heads, one query each 94 us (537 MB, 5.7 TB/s, 0.87 of
+// the copy rate); 64 of 100 to 8192 tokens 101 us (0.85).  With 138 query rows for each kv head it
+// comes to 178 TFLOP/s (8 sequences of 16384 tokens, 104 us): two warps a scheduler, which is what the
 // registers leave, do not hide one another's latencies.
 #include "kv8.cuh"
 

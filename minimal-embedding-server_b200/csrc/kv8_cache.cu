@@ -147,8 +147,8 @@ __device__ __forceinline__ float run_max(float v, float* red) {
 // run re-rounded when s grew, new tokens rounded once.  s_old counts only where the run already
 // held tokens.  Non-finite inputs do not set the scale: an infinity saturates, NaN becomes 0.
 // Each new value is read once and kept in registers between the maximum and the rounding.
-// Measured: 20 x 1000 tokens of 8 heads 28.3 us (123 MB, 4.3 TB/s, 0.66 of the copy rate, with 73% of the
-// issue slots taken); one token for each of 32 sequences 2.9 us.
+// Measured: 20 x 1000 tokens of 8 heads 26.3 us by itself, 28.3 with the read-back between (123 MB, 4.3 to 4.7 TB/s,
+// 0.66 to 0.71 of the copy rate, with 73% of the issue slots taken); one token for each of 32 sequences 2.8 us.
 template <int kKind, int P>
 __global__ void __launch_bounds__(Shape<P>::kThreads)
 kv8_append_kernel(const __nv_bfloat16* __restrict__ Kn, int64_t ldk, const __nv_bfloat16* __restrict__ Vn,
