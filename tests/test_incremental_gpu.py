@@ -226,3 +226,19 @@ def test_refusals(qwen3):
         IncrementalEmbedder(worker.model, 4, dtype=torch.float16)
     with pytest.raises(ValueError):
         IncrementalEmbedder(worker.model, 4, budget=10, recent=11)
+
+
+def test_more_texts_than_one_attention_call(qwen3):
+    """1100 forks of a text, some with two tokens more and some with one, against the same extensions in a short list."""
+    worker, _ = qwen3
+    rng = np.random.default_rng(14)
+    emb = IncrementalEmbedder(worker.model, num_pages=2400, page_size=16)
+    (h,), _ = emb.add([_ids(rng, 20)])
+    new = [[7], [5, 9]]
+    want = torch.stack([emb.extend(emb.fork(h, 1), [t])[0] for t in new])
+    got = emb.extend(emb.fork(h, 1100), [new[i % 3 == 0] for i in range(1100)])
+    assert got.shape == (1100, want.shape[1])
+    # the long list takes the GEMMs, the short ones the matrix-vector products
+    pick = torch.tensor([int(i % 3 == 0) for i in range(1100)], device=DEV)
+    assert (_cos(got.cpu().numpy(), want[pick].cpu().numpy()) > 0.9995).all()
+    assert _C.take_device_error() == 0
